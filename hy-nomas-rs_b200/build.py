@@ -28,7 +28,7 @@ SOURCES = ["kernels_commit.cu", "kernels_gather.cu", "kernels_qvg.cu", "kernels_
            "kernels_attn.cu",
            "bank.cpp", "abi.cpp",
            "noalloc.cu"]
-HEADERS = ["nkv_kernels.h", "nkv_device.cuh", "nkv_quant.cuh", "nkv_policy.h", "bank.h"]
+HEADERS = ["nkv_kernels.h", "nkv_device.cuh", "nkv_quant.cuh", "nkv_tcgen05.cuh", "nkv_policy.h", "bank.h"]
 
 # -fmad=false / -ffp-contract=off: the reference rounds every multiply and
 # add separately; the kernels ask for fused operations explicitly where the
