@@ -25,10 +25,11 @@ LIB = os.path.join(PKG, "nomas_kv", "libnomas_kv.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 SOURCES = ["kernels_commit.cu", "kernels_gather.cu", "kernels_qvg.cu", "kernels_qvg_fit.cu", "kernels_project.cu",
-           "kernels_attn.cu",
-           "bank.cpp", "abi.cpp",
+           "kernels_attn.cu", "kernels_packed.cu", "kernels_rotary.cu", "kernels_norm.cu",
+           "bank.cpp", "abi.cpp", "abi_block.cpp",
            "noalloc.cu"]
-HEADERS = ["nkv_kernels.h", "nkv_device.cuh", "nkv_quant.cuh", "nkv_tcgen05.cuh", "nkv_policy.h", "bank.h"]
+HEADERS = ["nkv_kernels.h", "nkv_device.cuh", "nkv_quant.cuh", "nkv_tcgen05.cuh", "nkv_policy.h", "nkv_packed.h",
+           "bank.h"]
 
 # -fmad=false / -ffp-contract=off: the reference rounds every multiply and
 # add separately; the kernels ask for fused operations explicitly where the

@@ -258,4 +258,117 @@ cudaError_t launch_attend_int8(const AttnArgs& a, cudaStream_t s);
 cudaError_t launch_kv_project(const void* x, const void* wk, const void* wv, const KvProjectParams& p,
                               cudaStream_t stream);
 
+// ------------------------------------------------------ rotary positions ---
+constexpr int kRotaryMaxDim = 256;
+enum PosType : int { POS_I32 = 0, POS_I64 = 1, POS_F32 = 2 };
+// The positions of the tokens (n_axes per token) and, per rotated pair, its
+// axis and its frequency theta^(-2 i / dims[axis]).
+struct RopePositions {
+  const void* data;
+  int32_t dtype;
+  int32_t n_axes;
+  int32_t pairs;
+  uint8_t axis[kRotaryMaxDim / 2];
+  double freq[kRotaryMaxDim / 2];
+};
+cudaError_t launch_rope_tables(const RopePositions& p, uint64_t tokens, float* cos_out, float* sin_out,
+                               cudaStream_t s);
+// q or k: strides in elements; weight the (D) RMS-norm gain or null; heads 0
+// when absent.
+struct RotarySide {
+  const void* in;
+  void* out;
+  int64_t in_token, in_head, out_token, out_head;
+  const void* weight;
+  int32_t heads;
+  int32_t pad_;
+};
+struct RotaryParams {
+  RopePositions pos;
+  RotarySide side[2];
+  uint64_t tokens;
+  int32_t D;
+  int32_t interleaved;
+  int32_t norm;
+  float eps;
+  int32_t tokens_per_cta;  // set by the launcher
+};
+cudaError_t launch_rotary(RotaryParams a, int dtype, cudaStream_t s);
+
+// ---------------------------------------------------- gated residual norm ---
+enum NormKind : int { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
+constexpr int64_t kResidualNormMaxDim = 32768;
+// Strides in elements; every vector may be null (gate / weights: 1, scale /
+// shift: 0); the modulation rows are (mod_rows, dim) contiguous.
+struct ResidualNormParams {
+  const void* x;
+  const void* branch;
+  void* h_out;
+  void* y_out;
+  int64_t x_stride, branch_stride, h_stride, y_stride;
+  const void* post_weight;
+  const void* weight;
+  const void* gate;
+  const void* scale;
+  const void* shift;
+  const int32_t* mod_index;
+  uint64_t tokens;
+  int64_t dim;
+  int32_t mod_rows;
+  int32_t weight_dtype, mod_dtype;
+  int32_t post, norm;
+  float eps;
+  uint64_t rows_per_cta;  // set by the launcher
+};
+cudaError_t launch_residual_norm(const ResidualNormParams& a, int dtype, cudaStream_t s);
+
+// ------------------------------------------------------ packed attention ---
+constexpr int kPackedTileKeys = 128;
+constexpr int kPackedItemRows = 256;
+// One CTA's work: packed rows [row0, row0 + rows) of a sequence and key/value
+// head (row r = token r / G, query head kvh * G + r % G) over its 128-key
+// tiles [t_lo, t_hi); part_row < 0: the whole key range, else the first of
+// the item's rows in the partial buffers.
+struct PackedItem {
+  int32_t q_start, q_len;
+  int32_t k_start, k_len;
+  int32_t row0, rows;
+  int32_t kvh;
+  int32_t t_lo, t_hi;
+  int32_t part_row;
+};
+// A unit whose key range is split: `parts` items of `rows` rows each, their
+// partial rows consecutive from part_row.
+struct PackedUnit {
+  int32_t q_start, row0, rows, kvh;
+  int32_t part_row, parts;
+};
+struct PackedArgs {
+  const PackedItem* items;
+  const PackedUnit* units;
+  int32_t n_items, n_units, max_unit_rows;
+  int32_t H, G, D;
+  int32_t causal;
+  int32_t out_f32;
+  int64_t block;
+  const uint16_t* q;
+  int64_t q_token, q_head;  // strides in elements
+  const uint16_t* v;        // the scrubbed values are read back from here
+  int64_t v_token, v_head;
+  void* out;                // (rows, H, D) in the type of q, or f32
+  float* lse;               // [H][lse_head]
+  int64_t lse_head;
+  const float* hist_o;      // (rows, H, D) or null
+  const float* hist_lse;    // [H][hist_lse_head]
+  int64_t hist_lse_head;
+  float scale_log2;         // softmax scale x log2(e)
+  float* part_o;            // (part rows, D), unnormalised
+  float* part_ml;           // (max, sum) per part row, base 2
+  uint32_t* status;
+};
+// False when the driver's tensor-map encoder is unavailable or refuses the
+// key / value layout.
+bool launch_attend_packed(const PackedArgs& a, int dtype, const void* k, int64_t k_tokens, int64_t k_token,
+                          int64_t k_head, int kv_heads, cudaStream_t s, cudaError_t* err);
+
 }  // namespace nkv

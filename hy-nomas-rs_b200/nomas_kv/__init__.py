@@ -28,8 +28,21 @@ __all__ = [
     "HistorySampling", "CacheStorage", "QvgConfig", "CacheConfig", "SegmentKv", "SegmentLayout", "CacheMetrics",
     "KvBank", "LayerCache", "build_cache", "history_frame_indices", "uniform_frame_indices",
     "recent_mix_uniform_frame_indices", "temporal_context_frame_indices", "plan_recent_trim", "partition_layers",
-    "lib",
+    "lib", "RotaryAxes", "rope_tables", "rotary", "residual_norm", "AttendPlan", "attend_packed",
 ]
+
+# the operators of block.py, imported at their first use: they need torch,
+# which the cache API itself only imports when a call does
+_BLOCK = ("RotaryAxes", "rope_tables", "rotary", "residual_norm", "AttendPlan", "attend_packed")
+
+
+def __getattr__(name):
+    if name in _BLOCK:
+        from . import block
+        for n in _BLOCK:
+            globals()[n] = getattr(block, n)
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 # ------------------------------------------------------------------ errors
@@ -353,6 +366,26 @@ class LayerCache:
         _check(lib().nkv_bank_attend_history(b._h, self._layer, C.c_void_p(q.data_ptr()), n, s,
                                              C.c_void_p(out.data_ptr()), C.c_void_p(lse.data_ptr())))
         return out, lse
+
+    def attend(self, plan, q, k, v, scale: Optional[float] = None, out=None, lse=None):
+        """The layer's whole attention of the current queries
+        (modules/attention.rs:143-189): softmax over this layer's history,
+        which every query sees, and the current segment's k / v as `plan` (an
+        AttendPlan) masks them.  q (plan.q_tokens, H, 128), k / v
+        (plan.k_tokens, H / group, 128) bf16 on the bank's device and stream;
+        returns (out, lse) of attend_packed.  The history part runs through
+        attend_history and its conditions apply (INT8 storage); an empty
+        history leaves the current segment alone."""
+        from . import block
+        b = self._bank
+        if plan.heads != b.heads or plan.head_dim != b.head_dim:
+            raise GeometryError(f"the plan must have {b.heads} heads of {b.head_dim}")
+        torch = _torch()
+        with torch.cuda.stream(b.stream):
+            history = None
+            if self.valid_len():
+                history = self.attend_history(q, scale)
+            return block.attend_packed(plan, q, k, v, scale=scale, history=history, out=out, lse=lse)
 
     # QvgCodec::with_codebooks (qvg.rs:101-104) / codebooks readback
     def set_qvg_codebooks(self, cb) -> None:

@@ -28,6 +28,8 @@ NKV_KERNEL_SEGMENT_DECODE = 4
 NKV_KERNEL_QVG_FIT = 5
 NKV_KERNEL_ATTEND = 6
 NKV_KERNEL_COUNT = 7
+NKV_POS_I32, NKV_POS_I64, NKV_POS_F32 = 0, 1, 2
+NKV_NORM_NONE, NKV_NORM_RMS, NKV_NORM_LAYER = 0, 1, 2
 KERNEL_NAMES = ("quantize", "float_archive", "qvg_encode", "gather", "segment_decode", "qvg_fit", "attend")
 NKV_NOALLOC_MAX_LAYERS = 64
 
@@ -130,6 +132,50 @@ class nkv_kv_project_args(C.Structure):
     ]
 
 
+class nkv_rope_axes(C.Structure):
+    _fields_ = [("n_axes", C.c_int32), ("dims", C.c_int32 * 4), ("interleaved", C.c_int32), ("theta", C.c_double)]
+
+
+class nkv_rotary_side(C.Structure):
+    _fields_ = [("in", C.c_void_p), ("out", C.c_void_p), ("in_token_stride", C.c_int64),
+                ("in_head_stride", C.c_int64), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("weight", C.c_void_p), ("heads", C.c_int32)]
+
+
+class nkv_rotary_args(C.Structure):
+    _fields_ = [("axes", nkv_rope_axes), ("positions", C.c_void_p), ("position_type", C.c_int32),
+                ("dtype", C.c_int32), ("tokens", C.c_uint64), ("head_dim", C.c_int32), ("norm", C.c_int32),
+                ("eps", C.c_float), ("q", nkv_rotary_side), ("k", nkv_rotary_side)]
+
+
+class nkv_residual_norm_args(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_uint64), ("dim", C.c_int64), ("dtype", C.c_int32), ("weight_dtype", C.c_int32),
+        ("mod_dtype", C.c_int32), ("post", C.c_int32), ("norm", C.c_int32), ("eps", C.c_float),
+        ("x", C.c_void_p), ("branch", C.c_void_p), ("h_out", C.c_void_p), ("y_out", C.c_void_p),
+        ("x_stride", C.c_int64), ("branch_stride", C.c_int64), ("h_stride", C.c_int64), ("y_stride", C.c_int64),
+        ("post_weight", C.c_void_p), ("weight", C.c_void_p), ("gate", C.c_void_p), ("scale", C.c_void_p),
+        ("shift", C.c_void_p), ("mod_index", C.c_void_p), ("mod_rows", C.c_int32),
+    ]
+
+
+class nkv_attend_plan_info(C.Structure):
+    _fields_ = [("q_tokens", C.c_uint64), ("k_tokens", C.c_uint64), ("items", C.c_uint64),
+                ("split_units", C.c_uint64), ("workspace_bytes", C.c_uint64)]
+
+
+class nkv_attend_args(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("out_dtype", C.c_int32), ("q_rows", C.c_uint64), ("k_rows", C.c_uint64),
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+        ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("scale", C.c_float), ("out", C.c_void_p), ("lse", C.c_void_p), ("hist_out", C.c_void_p),
+        ("hist_lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64),
+    ]
+
+
 P = C.c_void_p
 U64 = C.c_uint64
 I64 = C.c_int64
@@ -178,6 +224,17 @@ SIGNATURES = {
     "nkv_qvg_decode": (C.c_int, [P, I32, P, P, U64, I64, I64, I32, I32, I32, P, P]),
     "nkv_synth_fill": (C.c_int, [P, I32, U64, I64, I64, U64, U64, P, P, P]),
     "nkv_kv_project": (C.c_int, [C.POINTER(nkv_kv_project_args), P]),
+    "nkv_rope_tables": (C.c_int, [C.POINTER(nkv_rope_axes), P, I32, U64, P, P, P]),
+    "nkv_rotary": (C.c_int, [C.POINTER(nkv_rotary_args), P]),
+    "nkv_residual_norm": (C.c_int, [C.POINTER(nkv_residual_norm_args), P]),
+    "nkv_attend_plan_create": (C.c_int, [C.POINTER(U64), C.POINTER(U64), U64, I32, I32, I32, I32, U64, I32,
+                                         C.POINTER(P)]),
+    "nkv_attend_plan_destroy": (C.c_int, [P]),
+    "nkv_attend_plan_get_info": (C.c_int, [P, C.POINTER(nkv_attend_plan_info)]),
+    "nkv_attend_plan_status": (C.c_int, [P, C.POINTER(C.c_uint32)]),
+    "nkv_attend_schedule": (C.c_int, [C.POINTER(U64), C.POINTER(U64), U64, I32, I32, I32, U64, I32, P, U64,
+                                      C.POINTER(U64)]),
+    "nkv_attend_packed": (C.c_int, [P, C.POINTER(nkv_attend_args), P]),
     "nkv_int8_quantize_layers_noalloc": (C.c_int, [C.POINTER(P), C.POINTER(P), I32, I32, U64, I64, C.POINTER(P),
                                                    C.POINTER(P), C.POINTER(P), C.POINTER(P),
                                                    C.POINTER(C.c_uint32), P]),

@@ -440,6 +440,164 @@ typedef struct {
 } nkv_kv_project_args;
 int nkv_kv_project(const nkv_kv_project_args* args, void* stream);
 
+/* --------------------------------------- the attention block beside the cache --
+ * What a layer does around the cache in a turn (modules/attention.rs:107-189,
+ * norm.rs, rope.rs, modulate.rs): no counterpart in the reference's cache API.
+ * All three operators run on `stream` on the current device, read their
+ * inputs and write their outputs once, and synchronise nothing; they may be
+ * captured into a CUDA graph. */
+
+/* Rotary positions with several axes.  Axis a (1 to 4 of them: time, height,
+ * width, say) owns dims[a] (even, positive) of the rotated R = sum(dims)
+ * values of a head, in order; pair i of axis a turns by pos[a] * theta^(-2 i /
+ * dims[a]).  interleaved: pair p is the values (2p, 2p + 1), the layout of
+ * rope.rs:257-306 and nkv_kv_project; else (p, p + R / 2).  Values at and past
+ * R pass through. */
+typedef struct {
+  int32_t n_axes;
+  int32_t dims[4];
+  int32_t interleaved;
+  double theta;
+} nkv_rope_axes;
+
+/* Element type of positions, a (tokens, n_axes) array in device memory.
+ * Angles are formed and reduced in f64. */
+typedef enum { NKV_POS_I32 = 0, NKV_POS_I64 = 1, NKV_POS_F32 = 2 } nkv_position_type;
+
+/* cos / sin of every token's R / 2 angles, (tokens, R / 2) f32: the tables of
+ * nkv_kv_project when R is 128. */
+int nkv_rope_tables(const nkv_rope_axes* axes, const void* positions, int32_t position_type, uint64_t tokens,
+                    float* cos_out, float* sin_out, void* stream);
+
+/* One of the tensors nkv_rotary turns: (tokens, heads, D) with strides in
+ * elements and the last dimension dense; out may be in itself.  weight: the
+ * (D) RMS-norm gain in the tensor's type, or NULL. */
+typedef struct {
+  const void* in;
+  void* out;
+  int64_t in_token_stride, in_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  const void* weight;
+  int32_t heads;
+} nkv_rotary_side;
+typedef struct {
+  nkv_rope_axes axes;
+  const void* positions;
+  int32_t position_type;
+  int32_t dtype;     /* of q, k and the gains: F32, BF16 or F16 */
+  uint64_t tokens;   /* < 2^31 */
+  int32_t head_dim;  /* even, 2 to 256, at least R */
+  int32_t norm;      /* nonzero: x / sqrt(mean x^2 + eps) * weight per head first */
+  float eps;
+  nkv_rotary_side q;
+  nkv_rotary_side k; /* heads 0: no k */
+} nkv_rotary_args;
+/* Rotate q and k by their tokens' positions, after an RMS norm over head_dim
+ * when `norm` is set; f32 arithmetic, rounded once (nkv_kv_project, like the
+ * reference, also rounds between norm and rotation). */
+int nkv_rotary(const nkv_rotary_args* args, void* stream);
+
+/* Norm kinds: none; v / sqrt(mean v^2 + eps); (v - mean) / sqrt(var + eps). */
+typedef enum { NKV_NORM_NONE = 0, NKV_NORM_RMS = 1, NKV_NORM_LAYER = 2 } nkv_norm_kind;
+
+/* The residual stream between two blocks:
+ *   h = x + gate * (post(branch) * post_weight)
+ *   y = norm(h) * weight * (1 + scale) + shift
+ * x, branch, h_out, y_out: (tokens, dim) of `dtype`, row strides in elements;
+ * branch NULL: h = x and h_out is not written; norm NONE: y is not computed.
+ * h_out or y_out may be x or branch itself.  weights (dim) in weight_dtype, gate / scale / shift
+ * (mod_rows, dim) in mod_dtype (F32 or dtype each), any of them NULL (1, 1, 0).
+ * mod_index (tokens) i32 in device memory picks each token's row; NULL: row 0.
+ * A token whose index is outside [0, mod_rows) gets rows of NaN.  f32
+ * arithmetic; y comes from the unrounded h. */
+typedef struct {
+  uint64_t tokens;   /* < 2^31 */
+  int64_t dim;       /* 1 to 32768 */
+  int32_t dtype, weight_dtype, mod_dtype;
+  int32_t post, norm; /* nkv_norm_kind */
+  float eps;
+  const void* x;
+  const void* branch;
+  void* h_out;
+  void* y_out;
+  int64_t x_stride, branch_stride, h_stride, y_stride;
+  const void* post_weight;
+  const void* weight;
+  const void* gate;
+  const void* scale;
+  const void* shift;
+  const int32_t* mod_index;
+  int32_t mod_rows;
+} nkv_residual_norm_args;
+int nkv_residual_norm(const nkv_residual_norm_args* args, void* stream);
+
+/* Packed attention: n sequences, q_lens[s] query tokens over k_lens[s] keys
+ * each (0 allowed), packed one after another; `heads` query heads in groups
+ * of heads / kv_heads per key/value head (query head h reads key/value head
+ * h / (heads / kv_heads)).  Key j is visible to token i of its sequence iff
+ * j < lim(i): k_len when causal is 0; else ((i + k_len - q_len) / block + 1) *
+ * block, at most k_len, and 0 when i + k_len - q_len < 0 (block 1: ordinary
+ * causal, aligned to the last token; block = tokens per frame: a token sees
+ * its frame and those before it).
+ *
+ * A plan holds the work list for one set of lengths on one device; it is
+ * immutable but for its status word, and may serve any number of calls, on
+ * several streams at once.  It must outlive the calls and graphs that use
+ * it. */
+typedef struct nkv_attend_plan nkv_attend_plan;
+typedef struct {
+  uint64_t q_tokens, k_tokens; /* sums of the lengths */
+  uint64_t items, split_units; /* work items; rows blocks whose keys are split */
+  uint64_t workspace_bytes;    /* device memory nkv_attend_packed needs, 0 when nothing is split */
+} nkv_attend_plan_info;
+int nkv_attend_plan_create(const uint64_t* q_lens, const uint64_t* k_lens, uint64_t n, int32_t heads,
+                           int32_t kv_heads, int32_t head_dim, int32_t causal, uint64_t block, int32_t device,
+                           nkv_attend_plan** out);
+int nkv_attend_plan_destroy(nkv_attend_plan* plan);
+int nkv_attend_plan_get_info(const nkv_attend_plan* plan, nkv_attend_plan_info* out);
+/* Waits for the plan's device and reads the status word: bit 0 is set for
+ * good once a bounded wait inside a call ran out (its outputs are then
+ * undefined). */
+int nkv_attend_plan_status(const nkv_attend_plan* plan, uint32_t* status);
+/* The plan's work list for `sms` SMs without a device: per item {sequence
+ * start in q, in k, first packed row, rows, key/value head, first tile, last
+ * tile + 1, first partial row or -1}; min(*n, cap) items written. */
+int nkv_attend_schedule(const uint64_t* q_lens, const uint64_t* k_lens, uint64_t n, int32_t heads, int32_t kv_heads,
+                        int32_t causal, uint64_t block, int32_t sms, int64_t* out /* [cap][8] */, uint64_t cap,
+                        uint64_t* n_items);
+
+/* q (q_rows, heads, D), k / v (k_rows, kv_heads, D) of `dtype` (BF16 or F16),
+ * strides in elements, the last dimension dense, 16-byte aligned (strides
+ * multiples of 8 elements); D a multiple of 8 up to 128.  out (q_rows, heads,
+ * D) dense, of `dtype` or F32; lse (heads, q_rows) f32, the natural-log
+ * log-sum-exp of each row's scaled scores (-inf, with out 0, for a row that
+ * sees no key).  q_rows / k_rows may exceed the plan's tokens: rows behind the
+ * last sequence are not read or written.  hist_out (q_rows, heads, D) f32 and
+ * hist_lse (heads, q_rows) f32, both or neither: the normalised output and
+ * log-sum-exp over other keys (nkv_bank_attend_history), merged into out and
+ * lse.  workspace: workspace_bytes of device memory, 16-byte aligned, used by
+ * this call alone until its work is done.  Values of masked keys have no
+ * effect, non-finite ones included.  The probabilities are rounded to dtype
+ * before they meet V; everything else is f32. */
+typedef struct {
+  int32_t dtype, out_dtype;
+  uint64_t q_rows, k_rows;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_token_stride, q_head_stride;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  float scale; /* finite, positive */
+  void* out;
+  float* lse;
+  const float* hist_out;
+  const float* hist_lse;
+  void* workspace;
+  uint64_t workspace_bytes;
+} nkv_attend_args;
+int nkv_attend_packed(const nkv_attend_plan* plan, const nkv_attend_args* args, void* stream);
+
 /* Deterministic synthetic K/V for tests and benchmarks (no reference
  * counterpart): element (t, h, d) of a (rows = B*L, H, D) tensor is
  *   table[u >> 48] * (chan_scale ? chan_scale[h*D + d] : 1)
