@@ -324,18 +324,23 @@ cudaError_t launch_residual_norm(const ResidualNormParams& a, int dtype, cudaStr
 
 // ------------------------------------------------------ packed attention ---
 constexpr int kPackedTileKeys = 128;
+constexpr int kPackedStepKeys = 64;
 constexpr int kPackedItemRows = 256;
 // One CTA's work: packed rows [row0, row0 + rows) of a sequence and key/value
 // head (row r = token r / G, query head kvh * G + r % G) over its 128-key
 // tiles [t_lo, t_hi); part_row < 0: the whole key range, else the first of
-// the item's rows in the partial buffers.
-struct PackedItem {
+// the item's rows in the partial buffers.  steps0 / steps1: 64-key steps from
+// t_lo that rows 0-127 / 128-255 need; first_partial: the first tile, from
+// t_lo, that some row does not wholly see.
+struct alignas(16) PackedItem {
   int32_t q_start, q_len;
   int32_t k_start, k_len;
   int32_t row0, rows;
   int32_t kvh;
   int32_t t_lo, t_hi;
   int32_t part_row;
+  int32_t steps0, steps1, first_partial;
+  int32_t pad_[3];
 };
 // A unit whose key range is split: `parts` items of `rows` rows each, their
 // partial rows consecutive from part_row.

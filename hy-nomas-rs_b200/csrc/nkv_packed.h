@@ -94,6 +94,21 @@ inline double finish(const std::vector<Unit>& units, int64_t chunk, int sms) {
   return last + (split ? kMerge : 0.0);
 }
 
+// The steps of an item whose tile range is set.
+inline void set_steps(PackedItem* it, int64_t G, bool causal, int64_t block) {
+  auto limit = [&](int64_t row) { return packed_key_limit(it->q_len, it->k_len, causal, block, row / G); };
+  auto steps = [&](int64_t first, int64_t rows) -> int32_t {
+    if (rows <= 0) return 0;
+    const int64_t lim = std::min<int64_t>(limit(it->row0 + first + rows - 1), int64_t(it->t_hi) * kPackedTileKeys) -
+                        int64_t(it->t_lo) * kPackedTileKeys;
+    return int32_t(std::max<int64_t>(0, (lim + kPackedStepKeys - 1) / kPackedStepKeys));
+  };
+  constexpr int kHalf = kPackedItemRows / 2;
+  it->steps0 = steps(0, std::min(kHalf, it->rows));
+  it->steps1 = steps(kHalf, it->rows - kHalf);
+  it->first_partial = int32_t(std::max<int64_t>(0, limit(it->row0) / kPackedTileKeys - it->t_lo));
+}
+
 }  // namespace packed_detail
 
 // The schedule for `sms` SMs.  Items of 256 rows share each K / V tile between
@@ -149,6 +164,7 @@ inline PackedSchedule packed_schedule(const std::vector<int64_t>& q_lens, const 
       out.items.push_back(it);
     }
   }
+  for (PackedItem& it : out.items) set_steps(&it, H / kv_heads, causal, block);
   std::stable_sort(out.items.begin(), out.items.end(),
                    [](const PackedItem& a, const PackedItem& b) { return a.t_hi - a.t_lo > b.t_hi - b.t_lo; });
   return out;
