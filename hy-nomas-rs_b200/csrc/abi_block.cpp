@@ -5,7 +5,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstring>
 #include <functional>
 #include <memory>
 #include <string>
@@ -27,9 +26,9 @@ struct nkv_attend_plan {
   int32_t H = 0, kv_heads = 0, D = 0, causal = 0;
   int64_t block = 1;
   uint64_t q_tokens = 0, k_tokens = 0, part_rows = 0;
-  int32_t n_items = 0, n_units = 0, max_unit_rows = 0;
-  unsigned char* table = nullptr;  // status word (64 bytes), items, units
-  size_t items_off = 64, units_off = 0;
+  int32_t n_items = 0, n_ctas = 0, n_units = 0, max_unit_rows = 0;
+  unsigned char* table = nullptr;  // status word (64 bytes), items, CTAs' first items, units
+  size_t items_off = 64, ctas_off = 0, units_off = 0;
   uint64_t workspace() const {  // partial rows, then their (max, sum)
     return part_rows * (uint64_t(D) * sizeof(float) + sizeof(float2));
   }
@@ -105,6 +104,8 @@ Lens check_lens(const uint64_t* q_lens, const uint64_t* k_lens, uint64_t n, int3
   if (n) need(q_lens, "q_lens"), need(k_lens, "k_lens");
   if (heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 65535)
     fail(NKV_ERR_GEOMETRY, "heads must be a positive multiple of kv_heads, at most 65535");
+  if (heads / kv_heads > nkv::kPackedHalfRows)
+    fail(NKV_ERR_GEOMETRY, "at most 128 query heads per key/value head");
   if (block < 1 || block >= (uint64_t(1) << 31)) fail(NKV_ERR_ARGUMENT, "block must be 1 to 2^31 - 1");
   // packed rows (tokens x group) and tile coordinates are 32-bit
   constexpr uint64_t kMax = (uint64_t(1) << 31) - 1024;
@@ -284,13 +285,18 @@ int nkv_attend_plan_create(const uint64_t* q_lens, const uint64_t* k_lens, uint6
     p->q_tokens = l.q_tokens, p->k_tokens = l.k_tokens;
     p->part_rows = uint64_t(s.part_rows);
     p->n_items = int32_t(s.items.size()), p->n_units = int32_t(s.units.size());
+    p->n_ctas = int32_t(s.cta_begin.size()) - 1;
     p->max_unit_rows = s.max_unit_rows;
-    const size_t items_bytes = s.items.size() * sizeof(nkv::PackedItem);
-    p->units_off = (p->items_off + items_bytes + 63) / 64 * 64;
-    std::vector<unsigned char> host(p->units_off + s.units.size() * sizeof(nkv::PackedUnit), 0);
-    if (items_bytes) std::memcpy(host.data() + p->items_off, s.items.data(), items_bytes);
-    if (!s.units.empty())
-      std::memcpy(host.data() + p->units_off, s.units.data(), s.units.size() * sizeof(nkv::PackedUnit));
+    auto after = [](size_t at, size_t bytes) { return (at + bytes + 63) / 64 * 64; };
+    p->ctas_off = after(p->items_off, s.items.size() * sizeof(nkv::PackedItem));
+    p->units_off = after(p->ctas_off, s.cta_begin.size() * sizeof(int32_t));
+    std::vector<unsigned char> host(after(p->units_off, s.units.size() * sizeof(nkv::PackedUnit)), 0);
+    std::copy_n(reinterpret_cast<const unsigned char*>(s.items.data()), s.items.size() * sizeof(nkv::PackedItem),
+                host.data() + p->items_off);
+    std::copy_n(reinterpret_cast<const unsigned char*>(s.cta_begin.data()), s.cta_begin.size() * sizeof(int32_t),
+                host.data() + p->ctas_off);
+    std::copy_n(reinterpret_cast<const unsigned char*>(s.units.data()), s.units.size() * sizeof(nkv::PackedUnit),
+                host.data() + p->units_off);
     cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&p->table), host.size());
     if (e == cudaSuccess) e = cudaMemcpy(p->table, host.data(), host.size(), cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
@@ -369,7 +375,8 @@ int nkv_attend_packed(const nkv_attend_plan* plan, const nkv_attend_args* a, voi
     nkv::PackedArgs p{};
     p.items = reinterpret_cast<const nkv::PackedItem*>(plan->table + plan->items_off);
     p.units = reinterpret_cast<const nkv::PackedUnit*>(plan->table + plan->units_off);
-    p.n_items = plan->n_items, p.n_units = plan->n_units, p.max_unit_rows = plan->max_unit_rows;
+    p.cta_begin = reinterpret_cast<const int32_t*>(plan->table + plan->ctas_off);
+    p.n_ctas = plan->n_ctas, p.n_units = plan->n_units, p.max_unit_rows = plan->max_unit_rows;
     p.H = plan->H, p.G = plan->H / plan->kv_heads, p.D = plan->D;
     p.causal = plan->causal;
     p.block = plan->block;
@@ -389,9 +396,9 @@ int nkv_attend_packed(const nkv_attend_plan* plan, const nkv_attend_args* a, voi
     p.part_ml = p.part_o ? p.part_o + plan->part_rows * uint64_t(plan->D) : nullptr;
     p.status = reinterpret_cast<uint32_t*>(plan->table);
     cudaError_t e = cudaSuccess;
-    if (!nkv::launch_attend_packed(p, a->dtype, a->k, int64_t(plan->k_tokens), a->k_token_stride, a->k_head_stride,
-                                   plan->kv_heads, static_cast<cudaStream_t>(stream), &e))
-      fail(NKV_ERR_CUDA, "the driver refused the key / value layout");
+    if (!nkv::launch_attend_packed(p, a->dtype, a->k, int64_t(plan->q_tokens), int64_t(plan->k_tokens),
+                                   a->k_token_stride, a->k_head_stride, static_cast<cudaStream_t>(stream), &e))
+      fail(NKV_ERR_CUDA, "the driver refused the layout of q, k or v");
     nkv::check_cuda(e, "packed attention launch");
   });
 }

@@ -16,25 +16,25 @@
 // Rows of one key/value head are packed: row r of a sequence is token r / G,
 // query head kvh * G + r % G (G = heads / kv_heads), so a group's heads share
 // every K / V tile and a single new token of a grouped model fills G rows.  A
-// work item is up to 256 rows (two halves of 128) of one sequence and
-// key/value head over a range of 128-key tiles; a plan made once per set of
-// lengths lists the items, longest first, and splits the key range of long
-// rows when there are too few items to fill the GPU (their partial rows are
-// merged by k_packed_combine).
+// work item is two halves of up to 128 rows (whole tokens) of one sequence and
+// key/value head over a range of 128-key tiles.  A plan made once per set of
+// lengths deals the items to persistent CTAs, one per SM, and splits the key
+// range of long rows when there are too few items to fill the GPU (their
+// partial rows are merged by k_packed_combine).
 //
-// Per tile: S_h = Q_h K^T and O_h += P_h V as tcgen05.mma (kind::f16, f32 in
-// TMEM), P written over S_h in TMEM as the A operand, the running maximum
-// moved only when a tile exceeds it by more than 8 (base 2).  Scores, maxima,
-// sums and O stay in f32; P is rounded to the type of V because the tensor
-// core takes both operands in one type (an error of half a step of that type
-// per probability, the size of the output's own rounding); the sum uses the
-// unrounded values.
+// Per step of 64 keys: S_h = Q_h K^T and O_h += P_h V as tcgen05.mma (kind::f16,
+// f32 in TMEM), P written over S_h in TMEM as the A operand, the running
+// maximum moved only when a step exceeds it by more than 8 (base 2).  Scores,
+// maxima, sums and O stay in f32; P is rounded to the type of V because the
+// tensor core takes both operands in one type (an error of half a step of that
+// type per probability, the size of the output's own rounding); the sum uses
+// the unrounded values.
 //
 // A key past a row's limit has P = 0, but 0 times an infinity or a NaN in its
-// V row is a NaN: V tiles that some row of the item does not wholly see are
-// scrubbed in shared memory first (rows past the sequence zeroed, non-finite
-// values zeroed and remembered), and rows that do see such a value get it
-// added to their output at the end.
+// V row is a NaN: the V rows that some but not all rows of an item see are
+// checked in shared memory first (non-finite values zeroed and remembered; V
+// rows that none sees zeroed), and rows that do see such a value get it added
+// to their output at the end.
 //
 // Every wait on an mbarrier gives up after 1 s, sets bit 0 of the plan's
 // status word, frees the TMEM and returns.
@@ -52,21 +52,23 @@ namespace nkv {
 using namespace tc;
 namespace {
 
-constexpr int PQ = 128;             // rows per half (TMEM lanes)
+constexpr int PQ = kPackedHalfRows;  // rows per half (TMEM lanes)
 constexpr int PK = kPackedTileKeys;  // keys per K / V tile
 constexpr int SK = kPackedStepKeys;  // keys per softmax step
-static_assert(PK == 128 && SK == 64, "");
+static_assert(PQ == 128 && PK == 128 && SK == 64, "");
 // warps 0-7 softmax (half = warp / 4), 8-9 MMA issue (one per half), 10 TMA, 11 V scrub
 constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kTmaWarp = 10, kScrubWarp = 11;
 constexpr int kThreads = 384;
 
-// Shared memory for head_dim <= DP: the two Q halves, then a ring of K / V
-// tiles (K_0 V_0 K_1 V_1 ...).
+// Shared memory for head_dim <= DP: the two Q halves, a ring of K tiles, a
+// ring of V tiles, 4 KB per softmax warp to turn rows into lines.
 template <int DP>
 struct Shape {
   static constexpr int kTile = (DP / 64) * HALF_BYTES;  // 128 rows x DP 16-bit values
-  static constexpr int kStages = DP == 128 ? 5 : 8;
-  static constexpr int kSmem = (2 + kStages) * kTile + 512 + 1024;
+  static constexpr int kStages = DP == 128 ? 2 : 4;     // of each ring
+  static constexpr int kK = 2 * kTile, kV = kK + kStages * kTile, kStage = kV + kStages * kTile,
+                       kBars = kStage + kSoftmaxWarps * 4096;
+  static constexpr int kSmem = kBars + 512 + 1024;
   static_assert(kSmem <= 232448, "shared memory");
 };
 
@@ -106,8 +108,21 @@ __device__ __forceinline__ int key_limit(const PackedArgs& a, const PackedItem& 
   if (!a.causal) return it.k_len;
   const int64_t p = int64_t(i) + it.k_len - it.q_len;
   if (p < 0) return 0;
-  const int64_t lim = a.block == 1 ? p + 1 : (p / a.block + 1) * a.block;
+  const int64_t lim = a.block == 1 ? p + 1 : (int64_t(uint32_t(p) / uint32_t(a.block)) + 1) * a.block;
   return lim < it.k_len ? int(lim) : it.k_len;
+}
+
+// An item read anew: its fields need no registers while the steps run.
+__device__ __forceinline__ PackedItem read_item(const PackedItem* p) {
+  PackedItem it;
+  static_assert(sizeof(PackedItem) == 64, "");
+  int32_t* w = reinterpret_cast<int32_t*>(&it);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    asm volatile("ld.global.nc.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[4 * k]), "=r"(w[4 * k + 1]), "=r"(w[4 * k + 2]), "=r"(w[4 * k + 3])
+                 : "l"(reinterpret_cast<const int4*>(p) + k));
+  return it;
 }
 
 template <int DT>
@@ -146,14 +161,14 @@ __device__ __forceinline__ float max2_nan(float a, float b) {
   return d;
 }
 
-// Non-finite 16-bit halves of w (exponent all ones).
+// Exponent all ones: the smallest pattern of a non-finite value without sign.
+template <int DT>
+constexpr uint32_t kNonFinite = DT == BF16 ? 0x7F80u : 0x7C00u;
+// The non-finite 16-bit halves of w.
 template <int DT>
 __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {
-  constexpr uint32_t e = DT == BF16 ? 0x7F80u : 0x7C00u;
-  uint32_t m = 0u;
-  if ((w & e) == e) m |= 0xFFFFu;
-  if ((w & (e << 16)) == (e << 16)) m |= 0xFFFF0000u;
-  return m;
+  constexpr uint32_t e = kNonFinite<DT>;
+  return ((w & e) == e ? 0xFFFFu : 0u) | ((w & (e << 16)) == (e << 16) ? 0xFFFF0000u : 0u);
 }
 
 // Steps of 64 keys, two score buffers per half: TMEM columns
@@ -167,50 +182,36 @@ __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w) {
 // queue is short and an issuing warp stalls on it, so with one warp for both
 // halves the core stood still during that warp's waits (3,900 cycles per 128
 // keys at head_dim 128); two warps cover each other's.
+//
+// Between items nothing drains: the TMA warp brings the next item's first K
+// tile and, once the last scores are out, its Q; its first scores are computed
+// while the softmax warps still write the last output (its first PV waits for
+// that).  Counters run on across items, so every barrier's phases are seen in
+// turn by whoever waits on it.
 template <int DT, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_attend_packed(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+    k_attend_packed(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                    const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap hmap,
                     const PackedArgs a) {
   using Sh = Shape<DP>;
   constexpr int NST = Sh::kStages;
   extern __shared__ unsigned char packed_raw[];
   unsigned char* base =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(packed_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char* Qs = base;
-  unsigned char* Rs = base + 2 * Sh::kTile;  // the ring
-  // barriers: S full and P full (half, buffer); a half's last two PV done
-  // (once each); then per ring stage: full, empty, scrubbed, scrub wanted.
-  // A waiter sees every phase of a barrier in turn, never one early or late.
-  uint64_t* bars = reinterpret_cast<uint64_t*>(Rs + NST * Sh::kTile);
-  constexpr int kS = 0, kP = 4, kPv = 8, kFull = 12, kEmpty = kFull + NST, kClean = kFull + 2 * NST,
-                kGo = kFull + 3 * NST;
-  // tiles between two V tiles in the same stage, for the phases of the two
-  // scrub barriers (a stage is scrubbed again only after its last use was
-  // released, so neither side falls a phase behind)
-  constexpr int kVPeriod = NST % 2 ? NST : NST / 2;
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + kFull + 4 * NST);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(base + Sh::kBars);
+  // barriers: scores full and P full (half, buffer); a half's last two PV of
+  // an item done; Q full, Q free, O free (half); history full and read (half,
+  // columns); per K stage full and empty, per V stage full, scrubbed and empty
+  constexpr int kS = 0, kP = 4, kPv = 8, kQf = 12, kQe = 14, kOf = 16, kH = 18, kHr = 22, kKf = 26, kKe = kKf + NST,
+                kVf = kKe + NST, kVc = kVf + NST, kVe = kVc + NST, kBarCount = kVe + NST;
+  static_assert(kBarCount * 8 + 16 <= 512, "barriers");
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + kBarCount);
   volatile uint32_t* abort_flag = tslot + 1;
-  volatile uint32_t* dirty_flag = tslot + 2;
+  volatile uint32_t* dirty_flag = tslot + 2;  // some V value was zeroed in this CTA
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const PackedItem it = a.items[blockIdx.x];
   const int G = a.G;
+  const int first = a.cta_begin[blockIdx.x], last = a.cta_begin[blockIdx.x + 1];  // this CTA's items
   auto B = [&](int i) { return smem_addr(&bars[i]); };
-
-  const int n0 = it.steps0, n1 = it.steps1, nu = max(n0, n1);  // steps of the halves
-  const int n = (nu + 1) / 2;                                  // K / V tiles
-  const int first_partial = it.first_partial;  // tiles from this one on are not wholly visible to every row
-
-  // the TMA thread's load of ring entry idx (K_t, then V_t)
-  auto load_tile = [&](int idx) {
-    const int st = idx % NST;
-    bar_expect_tx(B(kFull + st), uint32_t(Sh::kTile));
-    const int tok = it.k_start + (it.t_lo + (idx >> 1)) * PK;
-#pragma unroll
-    for (int x = 0; x < DP / 64; ++x)
-      tma_tile(smem_addr(Rs + st * Sh::kTile) + uint32_t(x * HALF_BYTES), (idx & 1) ? &vmap : &kmap, 64 * x, it.kvh,
-               tok, B(kFull + st));
-    if ((idx & 1) && (idx >> 1) >= first_partial) bar_arrive(B(kGo + st));
-  };
 
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tslot))
@@ -218,51 +219,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 32 * kTmaWarp) {
-    for (int i = 0; i < 4; ++i) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(B(kS + i)) : "memory");
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(B(kP + i)), "r"(PQ / 32) : "memory");
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(B(kPv + i)) : "memory");
-    }
-    for (int i = 0; i < NST; ++i) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 32;" ::"r"(B(kClean + i)) : "memory");
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(B(kGo + i)) : "memory");
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(B(kFull + i)) : "memory");
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 2;" ::"r"(B(kEmpty + i)) : "memory");  // both MMA warps
+    // arrivals per phase: P, O free and history read by the half's 4 warps, K / V empty by both MMA warps, else 1
+    for (int i = 0; i < kBarCount; ++i) {
+      const bool by_half = (i >= kP && i < kP + 4) || (i >= kOf && i < kOf + 2) || (i >= kHr && i < kHr + 4);
+      const int count = by_half ? 4 : (i >= kKe && i < kKe + NST) || i >= kVe ? 2 : 1;
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(B(i)), "r"(count) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *abort_flag = 0u;
     *dirty_flag = 0u;
-    // the first K tile sets out beside Q; the others follow once Q has landed
-    if (n > 0) load_tile(0);
-  }
-  // Q: each softmax warp loads its 32 packed rows, consecutive lanes along a
-  // row (a row per thread would touch 32 lines with every load), zeros past the
-  // item's rows and past head_dim
-  if (warp < kSoftmaxWarps) {
-    unsigned char* Qh = Qs + (warp >> 2) * Sh::kTile;
-    constexpr int kLanes = DP / 8, kRows = 32 / kLanes;  // lanes per row, rows per round
-    const int c = lane % kLanes;
-    constexpr int kBatch = 8;  // loads in flight per lane
-#pragma unroll
-    for (int i0 = 0; i0 < 32; i0 += kRows * kBatch) {
-      uint4 v[kBatch];
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int j = warp * 32 + i0 + b * kRows + lane / kLanes;
-        v[b] = make_uint4(0u, 0u, 0u, 0u);
-        if (j < it.rows && 8 * c < a.D) {
-          const int r = it.row0 + j, tok = G == 1 ? r : r / G;
-          v[b] = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t(it.q_start) + tok) * a.q_token +
-                                                      int64_t(it.kvh * G + r - tok * G) * a.q_head) + c);
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const int j = warp * 32 + i0 + b * kRows + lane / kLanes;
-        *reinterpret_cast<uint4*>(Qh + swz(j & 127, c)) = v[b];
-      }
-    }
-    fence_async_smem();
   }
   tc_before();
   __syncthreads();
@@ -279,9 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The whole warp runs its half's schedule, so addresses stay warp-uniform;
     // one elected lane issues.
     const int hf = warp - kMmaWarp;
-    const int nh = hf ? n1 : n0;
-    const uint32_t dq = desc_k_lo(smem_addr(Qs + hf * Sh::kTile)), dr_k = desc_k_lo(smem_addr(Rs)),
-                   dr_v = desc_mn_lo(smem_addr(Rs));
+    const uint32_t dq = desc_k_lo(smem_addr(base + hf * Sh::kTile)), dk = desc_k_lo(smem_addr(base + Sh::kK)),
+                   dv = desc_mn_lo(smem_addr(base + Sh::kV));
     constexpr uint32_t kTileLo = Sh::kTile >> 4;
     const uint32_t s_tmem = tmem + uint32_t(hf * 128), o_tmem = tmem + uint32_t(256 + hf * 128);
     auto wait = [&](int i, uint32_t parity) {
@@ -293,251 +257,368 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_after();
       return r;
     };
-    // scores of step parity `odd` from ring stage st: keys 64 odd.. (8 groups of 8 rows)
-    auto s_mmas = [&](uint32_t odd, uint32_t st) {
-      const uint32_t b = dr_k + st * kTileLo + odd * uint32_t(8 * 1024 >> 4);
+    uint32_t tiles = 0, use0 = 0, use1 = 0;  // K / V tiles and uses of the score buffers so far
+    for (int i = first; i < last && ok; ++i) {
+      const PackedItem& it = a.items[i];
+      const int n0 = it.steps0, n1 = it.steps1, nh = hf ? n1 : n0, n = (max(n0, n1) + 1) / 2;
+      const uint32_t item_ph = uint32_t(i - first) & 1u;
+      // scores of step u: keys 64 (u & 1).. (8 groups of 8 rows) of the K tile in stage st
+      auto s_mmas = [&](int u, uint32_t st) {
+        const uint32_t odd = uint32_t(u) & 1u;
+        const uint32_t b = dk + st * kTileLo + odd * uint32_t(8 * 1024 >> 4);
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk)
-        mma_ss_lo(s_tmem + odd * SK, dq, b, uint32_t(((kk >> 2) * HALF_BYTES + (kk & 3) * 32) >> 4), kIdescS<DT>,
-                  kk > 0 ? 1u : 0u);
-      mma_commit(B(kS + 2 * hf + odd));
-    };
-    auto pv_mmas = [&](uint32_t odd, uint32_t st, uint32_t acc, int u) {
-      const uint32_t b = dr_v + st * kTileLo + odd * uint32_t(8 * 1024 >> 4);
+        for (int kk = 0; kk < DP / 16; ++kk)
+          mma_ss_lo(s_tmem + odd * SK, dq, b, uint32_t(((kk >> 2) * HALF_BYTES + (kk & 3) * 32) >> 4), kIdescS<DT>,
+                    kk > 0 ? 1u : 0u);
+        mma_commit(B(kS + 2 * hf + odd));
+        if (u == nh - 1) mma_commit(B(kQe + hf));  // Q has been read
+      };
+      auto pv_mmas = [&](int u, uint32_t st) {
+        const uint32_t odd = uint32_t(u) & 1u;
+        const uint32_t b = dv + st * kTileLo + odd * uint32_t(8 * 1024 >> 4);
 #pragma unroll
-      for (int kk = 0; kk < SK / 16; ++kk)
-        mma_ts_lo(o_tmem, s_tmem + odd * SK + uint32_t(kk * 8), b, uint32_t(kk * 2 * 1024 >> 4), kIdescO<DT, DP>,
-                  kk > 0 ? 1u : acc);
-      if (u >= nh - 2) mma_commit(B(kPv + 2 * hf + (u == nh - 1)));
-    };
-    // ring stage and phase of V_t; K_(t + 1) is the next
-    uint32_t v_st = 1, v_ph = 0;
-    if (nu > 0 && wait(kFull, 0)) {
+        for (int kk = 0; kk < SK / 16; ++kk)
+          mma_ts_lo(o_tmem, s_tmem + odd * SK + uint32_t(kk * 8), b, uint32_t(kk * 2 * 1024 >> 4), kIdescO<DT, DP>,
+                    (u > 0 || kk > 0) ? 1u : 0u);
+        if (u >= nh - 2) mma_commit(B(kPv + 2 * hf + (u == nh - 1)));
+      };
+      if (!wait(kQf + hf, item_ph)) break;
+      if (n > 0 && !wait(kKf + tiles % NST, (tiles / NST) & 1u)) break;
       if (elect_one()) {
-        if (nh > 0) s_mmas(0, 0);
-        if (nh > 1) s_mmas(1, 0);
-        mma_commit(B(kEmpty));
+        if (nh > 0) s_mmas(0, tiles % NST);
+        if (nh > 1) s_mmas(1, tiles % NST);
+        if (nh == 0) mma_commit(B(kQe + hf));
+        if (n > 0) mma_commit(B(kKe + tiles % NST));
       }
       __syncwarp();
-    }
-    // One round per tile; this half may need fewer steps than the other, but
-    // returns every stage to the ring.
-    for (int t = 0; t < n && ok; ++t) {
-      const int u = 2 * t;
-      const uint32_t ph = uint32_t(t) & 1u;
-      uint32_t kn_st = v_st + 1, kn_ph = v_ph;
-      if (kn_st == NST) kn_st = 0, kn_ph ^= 1u;
-      if (t >= first_partial) {
-        if (!wait(kClean + v_st, uint32_t((t - first_partial) / kVPeriod) & 1u)) break;
-      } else if (!wait(kFull + v_st, v_ph)) {
-        break;
+      // the first PV overwrites O, which the last item's output is read from
+      if (i > first && !wait(kOf + hf, item_ph ^ 1u)) break;
+      // One round per tile; this half may need fewer steps than the other, but
+      // returns every stage to the rings.
+      for (int t = 0; t < n && ok; ++t) {
+        const int u = 2 * t;
+        const uint32_t x = tiles + uint32_t(t), st = x % NST, next = (x + 1) % NST;
+        const bool more = t + 1 < n;
+        if (!wait(kVc + st, (x / NST) & 1u)) break;
+        if (more && !wait(kKf + next, ((x + 1) / NST) & 1u)) break;
+        if (u < nh && !wait(kP + 2 * hf, (use0 + uint32_t(t)) & 1u)) break;
+        if (elect_one()) {
+          if (u < nh) pv_mmas(u, st);
+          if (u + 2 < nh) s_mmas(u + 2, next);
+        }
+        __syncwarp();
+        if (u + 1 < nh && !wait(kP + 2 * hf + 1, (use1 + uint32_t(t)) & 1u)) break;
+        if (elect_one()) {
+          if (u + 1 < nh) pv_mmas(u + 1, st);
+          mma_commit(B(kVe + st));
+          if (u + 3 < nh) s_mmas(u + 3, next);
+          if (more) mma_commit(B(kKe + next));
+        }
+        __syncwarp();
       }
-      const bool more = t + 1 < n;
-      if (more && !wait(kFull + kn_st, kn_ph)) break;
-      if (u < nh && !wait(kP + 2 * hf, ph)) break;
-      if (elect_one()) {
-        if (u < nh) pv_mmas(0, v_st, t > 0 ? 1u : 0u, u);
-        if (u + 2 < nh) s_mmas(0, kn_st);
-      }
-      __syncwarp();
-      if (u + 1 < nh && !wait(kP + 2 * hf + 1, ph)) break;
-      if (elect_one()) {
-        if (u + 1 < nh) pv_mmas(1, v_st, 1u, u + 1);
-        mma_commit(B(kEmpty + v_st));
-        if (u + 3 < nh) s_mmas(1, kn_st);
-        if (more) mma_commit(B(kEmpty + kn_st));
-      }
-      __syncwarp();
-      v_st = kn_st + 1, v_ph = kn_ph;
-      if (v_st == NST) v_st = 0, v_ph ^= 1u;
+      tiles += uint32_t(n);
+      use0 += uint32_t(nh + 1) / 2;
+      use1 += uint32_t(nh) / 2;
     }
   } else if (warp == kTmaWarp) {
     // --------------------------------------------------------------- TMA
-    if (lane == 0 && n > 0) {
-      int idx = 1;
-      for (; idx < 2 * n; ++idx) {
-        if (idx >= NST && !bar_wait(B(kEmpty + idx % NST), uint32_t(idx / NST - 1) & 1u)) {
+    if (lane == 0) {
+      uint32_t kt = 0, vt = 0, slots = 0, hists = 0;  // K tiles, V tiles, V-ring slots, histories so far
+      uint32_t held = 0, parity = 0;  // per V stage (4 bits): free 0, a tile 1, history columns 2 + e; loads of e modulo 2
+      const uint32_t q_bytes = uint32_t(DP / 64) * uint32_t(a.half_rows) * 128u;
+      auto wait = [&](int i, uint32_t parity) {
+        if (ok && !bar_wait(B(i), parity)) fail();
+        return ok && *abort_flag == 0u;
+      };
+      auto load_k = [&](const PackedItem& it, int t) {
+        const uint32_t st = kt % NST;
+        if (kt >= NST && !wait(kKe + st, (kt / NST - 1) & 1u)) return false;
+        bar_expect_tx(B(kKf + st), uint32_t(Sh::kTile));
+#pragma unroll
+        for (int x = 0; x < DP / 64; ++x)
+          tma_tile(smem_addr(base + Sh::kK + st * Sh::kTile) + uint32_t(x * HALF_BYTES), &kmap, 64 * x, it.kvh,
+                   it.k_start + (it.t_lo + t) * PK, B(kKf + st));
+        ++kt;
+        return true;
+      };
+      // V tiles and history columns share the V ring (an item takes four
+      // history slots, a multiple of both ring lengths, so a V tile's stage
+      // stays its count modulo the length); a slot is free once what it held
+      // has been read: a tile by the MMA warps, history by the softmax warps
+      auto slot_free = [&](uint32_t st, uint32_t next) {
+        const uint32_t what = (held >> (4 * st)) & 15u;
+        held = (held & ~(15u << (4 * st))) | (next << (4 * st));
+        if (what == 0) return true;
+        if (what == 1) return wait(kVe + st, ((vt + NST - 1 - st) / NST - 1) & 1u);
+        return wait(kHr + what - 2, ((parity >> (what - 2)) & 1u) ^ 1u);
+      };
+      auto load_v = [&](const PackedItem& it, int t) {
+        const uint32_t st = slots % NST;
+        if (!slot_free(st, 1u)) return false;
+        bar_expect_tx(B(kVf + st), uint32_t(Sh::kTile));
+#pragma unroll
+        for (int x = 0; x < DP / 64; ++x)
+          tma_tile(smem_addr(base + Sh::kV + st * Sh::kTile) + uint32_t(x * HALF_BYTES), &vmap, 64 * x, it.kvh,
+                   it.k_start + (it.t_lo + t) * PK, B(kVf + st));
+        ++slots, ++vt;
+        return true;
+      };
+      // Q of item i: the box is the group's heads by half_rows / G tokens; rows
+      // behind the sequence belong to rows that are not kept
+      auto load_q = [&](int i) {
+        const PackedItem& it = a.items[i];
+        for (int hf = 0; hf < 2; ++hf) {
+          if (i > first && !wait(kQe + hf, uint32_t(i - first - 1) & 1u)) return false;
+          bar_expect_tx(B(kQf + hf), q_bytes);
+#pragma unroll
+          for (int x = 0; x < DP / 64; ++x)
+            tma_tile(smem_addr(base + hf * Sh::kTile) + uint32_t(x * HALF_BYTES), &qmap, 64 * x, it.kvh * G,
+                     it.q_start + (it.row0 + hf * a.half_rows) / G, B(kQf + hf));
+        }
+        return true;
+      };
+      auto load_history = [&](const PackedItem& it) {
+        for (int e = 0; e < 4; ++e) {  // half e / 2, columns (e & 1) * DP / 2
+          const uint32_t st = slots % NST;
+          if (!slot_free(st, 2u + uint32_t(e))) return false;
+          parity ^= 1u << e;
+          bar_expect_tx(B(kH + e), uint32_t(DP / 64) * uint32_t(a.half_rows) * 128u);
+#pragma unroll
+          for (int x = 0; x < DP / 64; ++x)
+            tma_tile(smem_addr(base + Sh::kV + st * Sh::kTile) + uint32_t(x * HALF_BYTES), &hmap,
+                     (e & 1) * (DP / 2) + 32 * x, it.kvh * G, it.q_start + (it.row0 + (e >> 1) * a.half_rows) / G,
+                     B(kH + e));
+          ++slots;
+        }
+        ++hists;
+        return true;
+      };
+      auto tiles_of = [&](const PackedItem& it) { return (max(it.steps0, it.steps1) + 1) / 2; };
+      if (first < last) {
+        if (tiles_of(a.items[first]) > 0) load_k(a.items[first], 0);
+        load_q(first);
+      }
+      int qs = first < last ? 1 : 0;
+      for (int i = first; i < last && ok; ++i) {
+        const PackedItem it = a.items[i];
+        const int n = tiles_of(it);
+        bool run = true;
+        for (int t = 0; t < n && run; ++t) run = load_v(it, t) && (t + 1 == n || load_k(it, t + 1));
+        if (run && i + 1 < last) {
+          run = (tiles_of(a.items[i + 1]) == 0 || load_k(a.items[i + 1], 0)) && load_q(i + 1);
+          qs += run;
+        }
+        if (run && a.hist_o && it.part_row < 0) run = load_history(it);
+        if (!run) break;
+      }
+      // no copy in flight when the CTA ends: wait (bounded) for the last load
+      // on every barrier; on the normal path they have all been consumed
+      for (uint32_t x = kt > NST ? kt - NST : 0; x < kt; ++x) bar_wait(B(kKf + x % NST), (x / NST) & 1u);
+      for (uint32_t x = vt > NST ? vt - NST : 0; x < vt; ++x) bar_wait(B(kVf + x % NST), (x / NST) & 1u);
+      if (qs)
+        for (int hf = 0; hf < 2; ++hf) bar_wait(B(kQf + hf), uint32_t(qs - 1) & 1u);
+      if (hists)
+        for (int e = 0; e < 4; ++e) bar_wait(B(kH + e), (hists - 1) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == kScrubWarp) {
+    // ----------------------------------------------------------- V scrub
+    uint32_t vt = 0;
+    for (int i = first; i < last && ok; ++i) {
+      const PackedItem& it = a.items[i];
+      const int n = (max(it.steps0, it.steps1) + 1) / 2, lo_vis = it.lo_vis, hi_vis = it.hi_vis;
+      for (int t = 0; t < n; ++t, ++vt) {
+        const uint32_t st = vt % NST;
+        if (!__all_sync(0xFFFFFFFFu, bar_wait(B(kVf + st), (vt / NST) & 1u))) {
           fail();
           break;
         }
-        if (*abort_flag) break;
-        load_tile(idx);
-      }
-      // no copy in flight when the CTA ends: wait (bounded) for the last
-      // load of every stage; on the normal path they have all been consumed
-      for (int u = max(0, idx - NST); u < idx; ++u) bar_wait(B(kFull + u % NST), uint32_t(u / NST) & 1u);
-    }
-    __syncwarp();
-  } else if (warp >= kScrubWarp) {
-    // ----------------------------------------------------------- V scrub
-    if (a.hist_o && it.part_row < 0) {
-      // the history rows that the end of the item reads, brought to L2
-      for (int i = lane; i < it.rows; i += 32) {
-        const int r = it.row0 + i, tok = r / G;
-        const float* src = a.hist_o + ((int64_t(it.q_start) + tok) * a.H + it.kvh * G + r - tok * G) * a.D;
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(a.D * 4) : "memory");
-      }
-    }
-    for (int t = first_partial; t < n; ++t) {
-      const int idx = 2 * t + 1, st = idx % NST;
-      // the load was issued, so the stage's earlier phases are over: without
-      // that its full barrier could still answer for the phase before them
-      if (!bar_wait(B(kGo + st), uint32_t((t - first_partial) / kVPeriod) & 1u) ||
-          !bar_wait(B(kFull + st), uint32_t(idx / NST) & 1u)) {
-        fail();
-        break;
-      }
-      const int left = it.k_len - (it.t_lo + t) * PK;  // rows of the tile that are keys
-      bool bad = false;
-      // whole 16-byte chunks, consecutive lanes on consecutive chunks, eight in flight
-      uint4* tile = reinterpret_cast<uint4*>(Rs + st * Sh::kTile);
-      for (int c0 = lane; c0 < Sh::kTile / 16; c0 += 32 * 8) {
-        uint4 v[8];
-#pragma unroll
-        for (int b = 0; b < 8; ++b) v[b] = tile[c0 + 32 * b];
-#pragma unroll
-        for (int b = 0; b < 8; ++b) {
-          const int c = c0 + 32 * b, row = (c >> 3) & 127;  // 8 chunks per row of a 64-column half
-          const uint32_t m0 = nonfinite_mask<DT>(v[b].x), m1 = nonfinite_mask<DT>(v[b].y),
-                         m2 = nonfinite_mask<DT>(v[b].z), m3 = nonfinite_mask<DT>(v[b].w);
-          if (row >= left) {
-            tile[c] = make_uint4(0u, 0u, 0u, 0u);
-          } else if (m0 | m1 | m2 | m3) {
-            bad = true;
-            tile[c] = make_uint4(v[b].x & ~m0, v[b].y & ~m1, v[b].z & ~m2, v[b].w & ~m3);
+        // rows [lo, hi) of the tile: seen by some rows of the item only; rows from hi on: by none
+        const int lo = max(0, min(PK, lo_vis - t * PK)), hi = max(0, min(PK, hi_vis - t * PK));
+        if (lo < PK) {
+          unsigned char* tile = base + Sh::kV + st * Sh::kTile;
+#pragma unroll 1
+          for (int x = 0; x < DP / 64; ++x, tile += HALF_BYTES) {
+            uint4* p = reinterpret_cast<uint4*>(tile);  // 8 chunks of 16 bytes per row, swizzled within the row
+            uint32_t top = 0u;
+            for (int c = 8 * lo + lane; c < 8 * hi; c += 32) {
+              const uint4 v = p[c];
+              top = __vmaxu2(__vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
+                                      __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)), top);
+            }
+            const bool bad = max(top & 0xFFFFu, top >> 16) >= kNonFinite<DT>;
+            if (__any_sync(0xFFFFFFFFu, bad)) {
+              *dirty_flag = 1u;
+              for (int c = 8 * lo + lane; c < 8 * hi; c += 32) {
+                const uint4 v = p[c];
+                p[c] = make_uint4(v.x & ~nonfinite_mask<DT>(v.x), v.y & ~nonfinite_mask<DT>(v.y),
+                                  v.z & ~nonfinite_mask<DT>(v.z), v.w & ~nonfinite_mask<DT>(v.w));
+              }
+            }
+            for (int c = 8 * hi + lane; c < 8 * PK; c += 32) p[c] = make_uint4(0u, 0u, 0u, 0u);
           }
+          fence_async_smem();
         }
+        __syncwarp();
+        arrive_lane0(B(kVc + st), lane);
       }
-      if (bad) *dirty_flag = 1u;
-      fence_async_smem();
-      bar_arrive(B(kClean + st));
-      if (*abort_flag) break;
     }
   } else {
     // ------------------------------------------------------------ softmax
     const int hf = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;
-    const int nh = hf ? n1 : n0;
+    const int row = (warp & 3) * 32 + lane;  // packed row of the half
     const uint32_t lane_q = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_cols = tmem + lane_q + uint32_t(hf * 128);
     const uint32_t o_cols = tmem + lane_q + uint32_t(256 + hf * 128);
-    const bool have = hf * PQ + row < it.rows;
-    const int r = it.row0 + hf * PQ + row, tok = have ? r / G : 0;
-    // visible keys, counted from the item's first tile
-    const int lim = have ? key_limit(a, it, tok) - it.t_lo * PK : 0;
-    float m = -INFINITY, l = 0.0f;
-    // Each phase of a step is a chain of latencies (TMEM, barriers), so the
-    // next step's barrier is tried before the second half of the exponentials
-    // and its scores are requested right after them, to arrive behind the end
-    // of this step.
-    float sv[SK];
-    auto request = [&](int u) {
-      tc_after();
-      tmem_load32_async(s_cols + (u & 1) * SK, sv);
-      tmem_load32_async(s_cols + (u & 1) * SK + 32, sv + 32);
-    };
-    // votes keep the warp together for the TMEM accesses
-    auto scores_full = [&](int u, bool tried) {
-      if (__all_sync(0xFFFFFFFFu, tried)) return true;
-      const bool r = __all_sync(0xFFFFFFFFu, bar_wait(B(kS + 2 * hf + (u & 1)), uint32_t(u >> 1) & 1u));
-      if (!r) fail();
-      return r;
-    };
-    if (nh > 0 && scores_full(0, false)) request(0);
-    for (int u = 0; u < nh && ok; ++u) {
-      const int buf = u & 1;
-      tmem_load_wait();
-      tmem_regs_after_wait(sv);
-      tmem_regs_after_wait(sv + 32);
-      const int vis = lim - u * SK;
-      if (__any_sync(0xFFFFFFFFu, vis < SK)) {
-#pragma unroll
-        for (int j = 0; j < SK; ++j)
-          if (j >= vis) sv[j] = -INFINITY;
+    // phases so far, one bit each: the score buffers (0, 1), the last PV and
+    // the one before (2, 3), the history (4); V tiles modulo the ring (5, 6)
+    uint32_t bits = 0;
+    for (int i = first; i < last && ok; ++i) {
+      int nh, lim;  // the half's steps; the row's visible keys, from the item's first tile
+      {
+        const PackedItem it = read_item(a.items + i);
+        nh = hf ? it.steps1 : it.steps0;
+        const int jt = int((uint32_t(row) * a.g_magic) >> 16);  // row / G
+        const bool have = row < min(a.half_rows, it.rows - hf * a.half_rows);
+        lim = have ? key_limit(a, it, (it.row0 + hf * a.half_rows) / G + jt) - it.t_lo * PK : 0;
+        const uint32_t tiles = uint32_t((max(it.steps0, it.steps1) + 1) / 2);
+        bits = (bits & 31u) | ((((bits >> 5) + tiles) & 3u) << 5);
       }
-      float mx[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) mx[c] = max2_nan(sv[c], sv[8 + c]);
-#pragma unroll
-      for (int j = 16; j < SK; j += 16)
-#pragma unroll
-        for (int c = 0; c < 8; ++c) mx[c] = max3_nan(mx[c], sv[j + c], sv[j + 8 + c]);
-      const float mt = max3_nan(max3_nan(mx[0], mx[1], mx[2]), max3_nan(mx[3], mx[4], mx[5]),
-                                max2_nan(mx[6], mx[7])) * a.scale_log2;
-      const bool move = mt > m + 8.0f;
-      const float mn = move ? mt : m;
-      const float alpha = move ? exp2f(m - mn) : 1.0f;  // 0 on a row's first visible step
-      // a row that has seen no key yet keeps m = -inf: its scores are all -inf
-      // and must give 0, not inf - inf
-      const float nm = mn == -INFINITY ? 0.0f : -mn;
-      const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(nm, nm);
-      float2 ls[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f),
-                      make_float2(0.0f, 0.0f)};
-      auto exponentiate = [&](int ch) {
-        uint32_t w[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int k0 = ch * 32 + 2 * j;
-          const float2 x = __ffma2_rn(make_float2(sv[k0], sv[k0 + 1]), sc2, nm2);
-          // a quarter of the exponentials on the FMA pipes, the others on the
-          // special-function unit, which alone would take 8 cycles each
-          const float2 p = j % 4 == 3 ? exp2_fma(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
-          ls[j & 3] = __fadd2_rn(ls[j & 3], p);
-          w[j] = pack2<DT>(p.x, p.y);
-        }
-        tmem_store16(s_cols + buf * SK + ch * 16, w);
-      };
-      exponentiate(0);
-      const bool next = u + 1 < nh;
-      const bool tried = next && bar_try(B(kS + 2 * hf + (buf ^ 1)), uint32_t((u + 1) >> 1) & 1u);
-      exponentiate(1);
-      if (next) {
-        if (!scores_full(u + 1, tried)) break;
-        request(u + 1);
-      }
-      const float2 l01 = __fadd2_rn(ls[0], ls[1]), l23 = __fadd2_rn(ls[2], ls[3]);
-      float lsum = (l01.x + l01.y) + (l23.x + l23.y);
-      if (!(mt < INFINITY)) lsum = __int_as_float(0x7FFFFFFF);  // a NaN or infinite score: the row is NaN
-      if (u > 0 && __any_sync(0xFFFFFFFFu, move)) {
-        // O_h's rows rescaled between PV_h(u - 1), which was issued before
-        // S_h(u + 1) and so is over, and PV_h(u), which waits for P_h(u)
-        if (!next && !__all_sync(0xFFFFFFFFu, bar_wait(B(kPv + 2 * hf), 0))) {
-          fail();
-          break;
-        }
+      float m = -INFINITY, l = 0.0f;
+      // Each phase of a step is a chain of latencies (TMEM, barriers), so the
+      // next step's barrier is tried before the second half of the exponentials
+      // and its scores are requested right after them, to arrive behind the end
+      // of this step.
+      float sv[SK];
+      auto request = [&](int u) {
         tc_after();
-#pragma unroll 1
-        for (int ch = 0; ch < DP / 32; ++ch) {
-          float ov[32];
-          tmem_load32(o_cols + ch * 32, ov);
+        tmem_load32_async(s_cols + (u & 1) * SK, sv);
+        tmem_load32_async(s_cols + (u & 1) * SK + 32, sv + 32);
+      };
+      auto s_phase = [&](int u) { return ((bits >> (u & 1)) ^ uint32_t(u >> 1)) & 1u; };
+      // votes keep the warp together for the TMEM accesses
+      auto scores_full = [&](int u, bool tried) {
+        if (__all_sync(0xFFFFFFFFu, tried)) return true;
+        const bool r = __all_sync(0xFFFFFFFFu, bar_wait(B(kS + 2 * hf + (u & 1)), s_phase(u)));
+        if (!r) fail();
+        return r;
+      };
+      bool before_seen = false;  // the last PV but one of this item
+      if (nh > 0 && scores_full(0, false)) request(0);
+      for (int u = 0; u < nh && ok; ++u) {
+        const int buf = u & 1;
+        tmem_load_wait();
+        tmem_regs_after_wait(sv);
+        tmem_regs_after_wait(sv + 32);
+        const int vis = lim - u * SK;
+        if (__any_sync(0xFFFFFFFFu, vis < SK)) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) ov[j] *= alpha;
-          tmem_store32(o_cols + ch * 32, ov);
+          for (int j = 0; j < SK; ++j)
+            if (j >= vis) sv[j] = -INFINITY;
         }
+        float mx[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) mx[c] = max2_nan(sv[c], sv[8 + c]);
+#pragma unroll
+        for (int j = 16; j < SK; j += 16)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) mx[c] = max3_nan(mx[c], sv[j + c], sv[j + 8 + c]);
+        const float mt = max3_nan(max3_nan(mx[0], mx[1], mx[2]), max3_nan(mx[3], mx[4], mx[5]),
+                                  max2_nan(mx[6], mx[7])) * a.scale_log2;
+        const bool move = mt > m + 8.0f;
+        const float mn = move ? mt : m;
+        const float alpha = move ? exp2f(m - mn) : 1.0f;  // 0 on a row's first visible step
+        // a row that has seen no key yet keeps m = -inf: its scores are all -inf
+        // and must not give inf - inf
+        const float nm = mn == -INFINITY ? 0.0f : -mn;
+        const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), nm2 = make_float2(nm, nm);
+        float2 ls[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f),
+                        make_float2(0.0f, 0.0f)};
+        auto exponentiate = [&](int ch) {
+          uint32_t w[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int k0 = ch * 32 + 2 * j;
+            const float2 x = __ffma2_rn(make_float2(sv[k0], sv[k0 + 1]), sc2, nm2);
+            // a quarter of the exponentials on the FMA pipes, the others on the
+            // special-function unit, which alone would take 8 cycles each
+            const float2 p = j % 4 == 3 ? exp2_fma(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
+            ls[j & 3] = __fadd2_rn(ls[j & 3], p);
+            w[j] = pack2<DT>(p.x, p.y);
+          }
+          tmem_store16(s_cols + buf * SK + ch * 16, w);
+        };
+        exponentiate(0);
+        const bool next = u + 1 < nh;
+        const bool tried = next && bar_try(B(kS + 2 * hf + (buf ^ 1)), s_phase(u + 1));
+        exponentiate(1);
+        if (next) {
+          if (!scores_full(u + 1, tried)) break;
+          request(u + 1);
+        }
+        const float2 l01 = __fadd2_rn(ls[0], ls[1]), l23 = __fadd2_rn(ls[2], ls[3]);
+        float lsum = (l01.x + l01.y) + (l23.x + l23.y);
+        if (!(mt < INFINITY)) lsum = __int_as_float(0x7FFFFFFF);  // a NaN or infinite score: the row is NaN
+        if (u > 0 && __any_sync(0xFFFFFFFFu, move)) {
+          // O_h's rows rescaled between PV_h(u - 1), which was issued before
+          // S_h(u + 1) and so is over, and PV_h(u), which waits for P_h(u)
+          if (!next) {
+            if (!__all_sync(0xFFFFFFFFu, bar_wait(B(kPv + 2 * hf), (bits >> 3) & 1u))) {
+              fail();
+              break;
+            }
+            before_seen = true;
+          }
+          tc_after();
+#pragma unroll 1
+          for (int ch = 0; ch < DP / 32; ++ch) {
+            float ov[32];
+            tmem_load32(o_cols + ch * 32, ov);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) ov[j] *= alpha;
+            tmem_store32(o_cols + ch * 32, ov);
+          }
+        }
+        tmem_store_wait();
+        l = l * alpha + lsum;
+        m = mn;
+        tc_before();
+        __syncwarp();
+        arrive_lane0(B(kP + 2 * hf + buf), lane);
       }
-      tmem_store_wait();
-      l = l * alpha + lsum;
-      m = mn;
-      tc_before();
-      __syncwarp();
-      arrive_lane0(B(kP + 2 * hf + buf), lane);
-    }
-    if (ok && nh > 0) {
-      // the half's last PV is done, and with it everything that read its Q
-      if (!__all_sync(0xFFFFFFFFu, bar_wait(B(kPv + 2 * hf + 1), 0))) fail();
-      tc_after();
-    }
-    if (__all_sync(0xFFFFFFFFu, ok && *abort_flag == 0u)) {
-      const int64_t q = int64_t(it.q_start) + tok;
-      const int h = it.kvh * G + (r - tok * G);
-      const bool whole = it.part_row < 0;
+      const PackedItem it = read_item(a.items + i);
+      bits ^= uint32_t((nh + 1) / 2) & 1u;
+      bits ^= (uint32_t(nh / 2) & 1u) << 1;
+      if (ok && nh > 0) {
+        bool r = nh < 2 || before_seen || bar_wait(B(kPv + 2 * hf), (bits >> 3) & 1u);
+        r = bar_wait(B(kPv + 2 * hf + 1), (bits >> 2) & 1u) && r;
+        if (!__all_sync(0xFFFFFFFFu, r)) fail();
+        bits ^= nh > 1 ? 12u : 4u;
+        tc_after();
+      }
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        ok = false;
+        break;
+      }
+      // ---- the item's output
+      const int row_tok = int((uint32_t(row) * a.g_magic) >> 16), row_head = row - row_tok * G;
+      const int n_rows = min(a.half_rows, it.rows - hf * a.half_rows);  // the half's rows
+      const bool have = row < n_rows;
+      const int64_t q = int64_t(it.q_start) + (it.row0 + hf * a.half_rows) / G + row_tok;
+      const int h = it.kvh * G + row_head;
+      const bool whole = it.part_row < 0, hist = a.hist_o && whole;
+      // the line (row of the output or of the partial buffers) of the half's
+      // first row; row j is j / G lines of H and j % G lines further
+      const int64_t line0 = whole ? q * a.H + h - (int64_t(row_tok) * a.H + row_head)
+                                  : int64_t(it.part_row) + hf * a.half_rows;
+      const int64_t line_tok = whole ? a.H : G;
       // normalisation and the history part's weights (base 2)
       float wo = 1.0f, wh = 0.0f;
       if (whole) {
         const float z = l > 0.0f || l != l ? m + log2f(l) : -INFINITY;  // NaN stays NaN
         wo = z == -INFINITY ? 0.0f : 1.0f / l;
         float lse2 = z;
-        if (a.hist_o && have) {
+        if (hist && have) {
           const float zh = __ldg(a.hist_lse + int64_t(h) * a.hist_lse_head + q) * 1.4426950408889634f;
           const float M = fmaxf(z, zh);
           if (M == -INFINITY) {
@@ -551,88 +632,100 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (have) a.lse[int64_t(h) * a.lse_head + q] = lse2 * 0.69314718055994531f;
       } else if (have) {
-        reinterpret_cast<float2*>(a.part_ml)[int64_t(it.part_row) + hf * PQ + row] = make_float2(m, l);
+        reinterpret_cast<float2*>(a.part_ml)[int64_t(it.part_row) + hf * a.half_rows + row] = make_float2(m, l);
       }
-      // The weighted rows leave through shared memory, DP / 2 columns at a
-      // time, so that consecutive lanes write consecutive bytes of a row: the
-      // warp's 32 rows in its quarter of the half's Q tile, 16-byte chunks
-      // XORed with the row.
-      constexpr int kCols = DP / 2, kLanes = kCols / 4, kRows = 32 / kLanes, kBatch = 8;
-      unsigned char* stage = Qs + hf * Sh::kTile + (warp & 3) * (32 * kCols * 4);
+      // The weighted rows leave through the warp's 4 KB, 128 bytes of each of
+      // its 32 rows at a time (64 16-bit values or 32 f32), 16-byte chunks XORed
+      // with the row, so that eight lanes write 128 consecutive bytes.
       const bool slow = *dirty_flag != 0u;
-      const int n_rows = min(32, it.rows - hf * PQ - (warp & 3) * 32);  // the warp's rows
-      const int64_t my_off = whole ? (q * a.H + h) * a.D : (int64_t(it.part_row) + hf * PQ + row) * a.D;
-      const int c = lane % kLanes;
+      const bool wide = !whole || a.out_f32;  // f32 rows
+      unsigned char* dst = whole ? static_cast<unsigned char*>(a.out) : reinterpret_cast<unsigned char*>(a.part_o);
+      const int esize = wide ? 4 : 2;
+      unsigned char* stage = base + Sh::kStage + warp * 4096;
 #pragma unroll 1
-      for (int c0 = 0; c0 < DP; c0 += kCols) {
-#pragma unroll 1
-        for (int ch = 0; ch < kCols; ch += 32) {
-          float ov[32];
-          __syncwarp();
-          if (nh > 0) tmem_load32(o_cols + c0 + ch, ov);
-          if (nh == 0 || l == 0.0f) {  // nothing visible here (the MMA, if any, ran on P = 0)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) ov[j] = 0.0f;
-          }
-          if (slow && have) {
-            // the scrubbed values of keys that this row does see
-            const int hi = min(lim, nh * SK);
-            for (int k = first_partial * PK; k < hi; ++k) {
-              const uint16_t* vr = a.v + (int64_t(it.k_start) + it.t_lo * PK + k) * a.v_token +
-                                   int64_t(it.kvh) * a.v_head + c0 + ch;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (c0 + ch + j < a.D) {
-                  const float x = dev::load_elem<DT>(vr, uint64_t(j));
-                  if (!(fabsf(x) <= 3.4e38f)) ov[j] += x;
-                }
-            }
-          }
-#pragma unroll
-          for (int d = 0; d < 8; ++d)
-            *reinterpret_cast<float4*>(stage + lane * (kCols * 4) + (((ch / 4 + d) ^ (lane & 7)) << 4)) =
-                make_float4(ov[4 * d] * wo, ov[4 * d + 1] * wo, ov[4 * d + 2] * wo, ov[4 * d + 3] * wo);
-        }
+      for (int c0 = 0; c0 < DP; c0 += 32) {
+        float ov[32];
         __syncwarp();
-        for (int i0 = 0; i0 < n_rows; i0 += kRows * kBatch) {
-          float4 o[kBatch], x[kBatch];
-          float w[kBatch];
-          int64_t off[kBatch];
+        if (nh > 0) tmem_load32(o_cols + c0, ov);
+        if (c0 + 32 == DP) {  // O may be overwritten
+          tc_before();
+          __syncwarp();
+          arrive_lane0(B(kOf + hf), lane);
+        }
+        if (nh == 0 || l == 0.0f) {  // nothing visible here (the MMA, if any, ran on P = 0)
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            const int j = i0 + b * kRows + lane / kLanes;
-            off[b] = __shfl_sync(0xFFFFFFFFu, my_off, j) + c0 + 4 * c;
-            w[b] = __shfl_sync(0xFFFFFFFFu, wh, j);
-            if (j >= n_rows || c0 + 4 * c >= a.D) off[b] = -1;
-            x[b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (off[b] >= 0 && w[b] != 0.0f) x[b] = __ldg(reinterpret_cast<const float4*>(a.hist_o + off[b]));
-            o[b] = *reinterpret_cast<const float4*>(stage + j * (kCols * 4) + ((c ^ (j & 7)) << 4));
-          }
-          if (a.hist_o) {
+          for (int j = 0; j < 32; ++j) ov[j] = 0.0f;
+        }
+        if (slow && have) {
+          // the zeroed values of keys that this row does see
+          const int hi = min(lim, nh * SK);
+          for (int k = it.lo_vis; k < hi; ++k) {
+            const uint16_t* vr = a.v + (int64_t(it.k_start) + it.t_lo * PK + k) * a.v_token +
+                                 int64_t(it.kvh) * a.v_head + c0;
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b)
-              if (w[b] != 0.0f) {
-                o[b].x = fmaf(x[b].x, w[b], o[b].x);
-                o[b].y = fmaf(x[b].y, w[b], o[b].y);
-                o[b].z = fmaf(x[b].z, w[b], o[b].z);
-                o[b].w = fmaf(x[b].w, w[b], o[b].w);
+            for (int j = 0; j < 32; ++j)
+              if (c0 + j < a.D) {
+                const float x = dev::load_elem<DT>(vr, uint64_t(j));
+                if (!(fabsf(x) <= 3.4e38f)) ov[j] += x;
               }
           }
-          if (!whole || a.out_f32) {
-            float* dst = whole ? static_cast<float*>(a.out) : a.part_o;
+        }
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b)
-              if (off[b] >= 0) *reinterpret_cast<float4*>(dst + off[b]) = o[b];
-          } else {
+        for (int j = 0; j < 32; ++j) ov[j] *= wo;
+        if (hist) {
+          constexpr int kCols = DP / 2;  // columns per history slot
+          const int e = c0 / kCols;
+          if (c0 % kCols == 0 && !__all_sync(0xFFFFFFFFu, bar_wait(B(kH + 2 * hf + e), (bits >> 4) & 1u))) {
+            fail();
+            break;
+          }
+          // its slots are behind the V tiles so far (and earlier histories,
+          // four slots each, a multiple of the ring's length)
+          const uint32_t st = ((bits >> 5) + uint32_t(2 * hf + e)) % NST;
+          if (wh != 0.0f) {
+            const unsigned char* src = base + Sh::kV + st * Sh::kTile + ((c0 % kCols) / 32) * HALF_BYTES + row * 128;
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b)
-              if (off[b] >= 0)
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + off[b]) =
-                    make_uint2(pack2<DT>(o[b].x, o[b].y), pack2<DT>(o[b].z, o[b].w));
+            for (int d = 0; d < 8; ++d) {
+              const float4 x = *reinterpret_cast<const float4*>(src + ((d ^ (row & 7)) << 4));
+              ov[4 * d] = fmaf(x.x, wh, ov[4 * d]);
+              ov[4 * d + 1] = fmaf(x.y, wh, ov[4 * d + 1]);
+              ov[4 * d + 2] = fmaf(x.z, wh, ov[4 * d + 2]);
+              ov[4 * d + 3] = fmaf(x.w, wh, ov[4 * d + 3]);
+            }
+          }
+          if ((c0 + 32) % kCols == 0) {  // read: back to the ring
+            __syncwarp();
+            arrive_lane0(B(kHr + 2 * hf + e), lane);
           }
         }
+        // into the staging rows
+        if (wide) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((d ^ (lane & 7)) << 4)) =
+                make_float4(ov[4 * d], ov[4 * d + 1], ov[4 * d + 2], ov[4 * d + 3]);
+        } else {
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((((c0 & 32) / 8 + d) ^ (lane & 7)) << 4)) =
+                make_uint4(pack2<DT>(ov[8 * d], ov[8 * d + 1]), pack2<DT>(ov[8 * d + 2], ov[8 * d + 3]),
+                           pack2<DT>(ov[8 * d + 4], ov[8 * d + 5]), pack2<DT>(ov[8 * d + 6], ov[8 * d + 7]));
+          if (!(c0 & 32)) continue;
+        }
+        // and out: lane / 8 the row within four, lane % 8 the 16 bytes
         __syncwarp();
+        const int c = (wide ? c0 : c0 - 32) + (lane & 7) * (16 / esize);  // first column of the 16 bytes
+        const bool col_ok = c < a.D;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int rr = 4 * k + (lane >> 3), j = (warp & 3) * 32 + rr;  // row of the warp, of the half
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+          const int jt = int((uint32_t(j) * a.g_magic) >> 16);  // j / G
+          const int64_t line = line0 + jt * line_tok + (j - jt * G);
+          if (j < n_rows && col_ok) *reinterpret_cast<uint4*>(dst + (line * a.D + c) * esize) = v;
+        }
       }
+      bits ^= hist ? 16u : 0u;
     }
   }
   tc_before();
@@ -711,29 +804,39 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return enc;
 }
 
-// (tokens, heads, D) with strides in elements as (values, head, token), boxes
-// of 64 values x 1 head x 128 tokens.
-bool make_kv_map(CUtensorMap* m, const void* base, int dt, int64_t tokens, int heads, int D, int64_t token_stride,
-                 int64_t head_stride) {
+// (tokens, heads, D) with strides in elements as (values, head, token); boxes
+// of 128 bytes of values x `box_heads` heads x `box_tokens` tokens, 128-byte
+// swizzled.  A key / value tile is one head by 128 tokens, half the rows of an
+// item are G heads by 128 / G tokens.
+bool make_map(CUtensorMap* m, const void* base, int dt, int64_t tokens, int heads, int D, int64_t token_stride,
+              int64_t head_stride, int box_heads, int box_tokens) {
   const PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
   if (!enc) return false;
+  const size_t es = dtype_size(dt);
   const cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(heads), cuuint64_t(tokens)};
   // a dimension of one element has no stride: give it a valid one
-  const cuuint64_t strides[2] = {cuuint64_t(heads > 1 ? head_stride : D) * 2,
-                                 cuuint64_t(tokens > 1 ? token_stride : int64_t(D) * heads) * 2};
-  const cuuint32_t box[3] = {64u, 1u, uint32_t(PK)};
+  const cuuint64_t strides[2] = {cuuint64_t(heads > 1 ? head_stride : D) * es,
+                                 cuuint64_t(tokens > 1 ? token_stride : int64_t(D) * heads) * es};
+  const cuuint32_t box[3] = {uint32_t(128 / es), uint32_t(box_heads), uint32_t(box_tokens)};
   const cuuint32_t estr[3] = {1u, 1u, 1u};
-  return enc(m, dt == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  const CUtensorMapDataType type = dt == F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dt == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(m, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+struct Maps {
+  CUtensorMap q, k, v, h;
+};
+
 template <int DT, int DP>
-cudaError_t launch_shape(const CUtensorMap& km, const CUtensorMap& vm, const PackedArgs& a, cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(k_attend_packed<DT, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kSmem);
+cudaError_t launch_shape(const Maps& m, const PackedArgs& a, cudaStream_t s) {
+  cudaError_t e = cudaFuncSetAttribute(k_attend_packed<DT, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Shape<DP>::kSmem);
   if (e != cudaSuccess) return e;
-  k_attend_packed<DT, DP><<<unsigned(a.n_items), kThreads, Shape<DP>::kSmem, s>>>(km, vm, a);
+  k_attend_packed<DT, DP><<<unsigned(a.n_ctas), kThreads, Shape<DP>::kSmem, s>>>(m.q, m.k, m.v, m.h, a);
   e = cudaGetLastError();
   if (e != cudaSuccess || a.n_units == 0) return e;
   k_packed_combine<DT><<<dim3(unsigned(a.n_units), unsigned((a.max_unit_rows + 7) / 8)), 256, 0, s>>>(a);
@@ -742,20 +845,26 @@ cudaError_t launch_shape(const CUtensorMap& km, const CUtensorMap& vm, const Pac
 
 }  // namespace
 
-bool launch_attend_packed(const PackedArgs& a, int dtype, const void* k, int64_t k_tokens, int64_t k_token,
-                          int64_t k_head, int kv_heads, cudaStream_t s, cudaError_t* err) {
+bool launch_attend_packed(PackedArgs a, int dtype, const void* k, int64_t q_tokens, int64_t k_tokens, int64_t k_token,
+                          int64_t k_head, cudaStream_t s, cudaError_t* err) {
   *err = cudaSuccess;
-  if (a.n_items == 0) return true;
-  CUtensorMap km{}, vm{};
-  if (k_tokens > 0) {  // no key at all: no item has a tile and the maps are never read
-    if (!make_kv_map(&km, k, dtype, k_tokens, kv_heads, a.D, k_token, k_head) ||
-        !make_kv_map(&vm, a.v, dtype, k_tokens, kv_heads, a.D, a.v_token, a.v_head))
-      return false;
-  }
+  if (a.n_ctas == 0) return true;
+  const int box_tokens = kPackedHalfRows / a.G;
+  a.half_rows = a.G * box_tokens;
+  a.g_magic = 65536u / uint32_t(a.G) + 1u;  // (j * g_magic) >> 16 = j / G for j < 128, G <= 128
+  Maps m{};
+  if (!make_map(&m.q, a.q, dtype, q_tokens, a.H, a.D, a.q_token, a.q_head, a.G, box_tokens)) return false;
+  // no key at all: no item has a tile and the maps are never read
+  if (k_tokens > 0 &&
+      (!make_map(&m.k, k, dtype, k_tokens, a.H / a.G, a.D, k_token, k_head, 1, kPackedTileKeys) ||
+       !make_map(&m.v, a.v, dtype, k_tokens, a.H / a.G, a.D, a.v_token, a.v_head, 1, kPackedTileKeys)))
+    return false;
+  if (a.hist_o && !make_map(&m.h, a.hist_o, F32, q_tokens, a.H, a.D, int64_t(a.H) * a.D, a.D, a.G, box_tokens))
+    return false;
   if (dtype == BF16)
-    *err = a.D <= 64 ? launch_shape<BF16, 64>(km, vm, a, s) : launch_shape<BF16, 128>(km, vm, a, s);
+    *err = a.D <= 64 ? launch_shape<BF16, 64>(m, a, s) : launch_shape<BF16, 128>(m, a, s);
   else
-    *err = a.D <= 64 ? launch_shape<F16, 64>(km, vm, a, s) : launch_shape<F16, 128>(km, vm, a, s);
+    *err = a.D <= 64 ? launch_shape<F16, 64>(m, a, s) : launch_shape<F16, 128>(m, a, s);
   return true;
 }
 

@@ -325,13 +325,13 @@ cudaError_t launch_residual_norm(const ResidualNormParams& a, int dtype, cudaStr
 // ------------------------------------------------------ packed attention ---
 constexpr int kPackedTileKeys = 128;
 constexpr int kPackedStepKeys = 64;
-constexpr int kPackedItemRows = 256;
-// One CTA's work: packed rows [row0, row0 + rows) of a sequence and key/value
-// head (row r = token r / G, query head kvh * G + r % G) over its 128-key
-// tiles [t_lo, t_hi); part_row < 0: the whole key range, else the first of
-// the item's rows in the partial buffers.  steps0 / steps1: 64-key steps from
-// t_lo that rows 0-127 / 128-255 need; first_partial: the first tile, from
-// t_lo, that some row does not wholly see.
+constexpr int kPackedHalfRows = 128;  // the TMEM lanes of a half; G * (128 / G) of them hold rows
+// One work item: packed rows [row0, row0 + rows) of a sequence and key/value
+// head (row r = token r / G, query head kvh * G + r % G), two halves of up to
+// half_rows, over its 128-key tiles [t_lo, t_hi); part_row < 0: the whole key
+// range, else the first of the item's rows in the partial buffers.  steps0 /
+// steps1: 64-key steps from t_lo that the halves need; keys below lo_vis,
+// from t_lo, are seen by every row, keys from hi_vis on by none.
 struct alignas(16) PackedItem {
   int32_t q_start, q_len;
   int32_t k_start, k_len;
@@ -339,8 +339,9 @@ struct alignas(16) PackedItem {
   int32_t kvh;
   int32_t t_lo, t_hi;
   int32_t part_row;
-  int32_t steps0, steps1, first_partial;
-  int32_t pad_[3];
+  int32_t steps0, steps1;
+  int32_t lo_vis, hi_vis;
+  int32_t pad_[2];
 };
 // A unit whose key range is split: `parts` items of `rows` rows each, their
 // partial rows consecutive from part_row.
@@ -349,16 +350,19 @@ struct PackedUnit {
   int32_t part_row, parts;
 };
 struct PackedArgs {
-  const PackedItem* items;
+  const PackedItem* items;      // by CTA
+  const int32_t* cta_begin;     // [n_ctas + 1]
   const PackedUnit* units;
-  int32_t n_items, n_units, max_unit_rows;
+  int32_t n_ctas, n_units, max_unit_rows;
   int32_t H, G, D;
+  int32_t half_rows;            // set by the launcher
+  uint32_t g_magic;             // set by the launcher
   int32_t causal;
   int32_t out_f32;
   int64_t block;
   const uint16_t* q;
   int64_t q_token, q_head;  // strides in elements
-  const uint16_t* v;        // the scrubbed values are read back from here
+  const uint16_t* v;        // the zeroed values are read back from here
   int64_t v_token, v_head;
   void* out;                // (rows, H, D) in the type of q, or f32
   float* lse;               // [H][lse_head]
@@ -372,8 +376,8 @@ struct PackedArgs {
   uint32_t* status;
 };
 // False when the driver's tensor-map encoder is unavailable or refuses the
-// key / value layout.
-bool launch_attend_packed(const PackedArgs& a, int dtype, const void* k, int64_t k_tokens, int64_t k_token,
-                          int64_t k_head, int kv_heads, cudaStream_t s, cudaError_t* err);
+// layout.
+bool launch_attend_packed(PackedArgs a, int dtype, const void* k, int64_t q_tokens, int64_t k_tokens, int64_t k_token,
+                          int64_t k_head, cudaStream_t s, cudaError_t* err);
 
 }  // namespace nkv
