@@ -11,44 +11,64 @@
 // round once, at their stores.
 //
 // The pass is bound by its bytes: x and branch read once, h and y written
-// once.  A row lives in the registers of one CTA; a CTA keeps the products
-// gate * post_weight and weight * (1 + scale) and the shift of the current
-// group in registers over a run of consecutive rows, because reading them
-// again per row (20 bytes a column from L2) would cost more than the row
-// itself.
+// once.  A row lives in the registers of one CTA, 16 columns a thread.  A CTA
+// takes a run of consecutive rows and keeps the products gate * post_weight
+// and weight * (1 + scale) and the shift of the current group in registers:
+// reading their five vectors anew for every row (20 bytes a column from L2)
+// would cost more than the row itself.  That leaves room for two CTAs an SM at
+// 5,120 columns, too few loads in flight for HBM if they went to registers as
+// well: rows arrive by cp.async, several ahead, each thread waiting for its own
+// bytes only.
+#include <algorithm>
+
 #include "nkv_device.cuh"
 #include "nkv_kernels.h"
 
 namespace nkv {
 namespace {
 
-// Element i of a vector that is f32 or the stream's 16-bit type.
+// One element by the hardware conversions (a NaN stays one, its payload does
+// not matter here).
 template <int DT>
-__device__ __forceinline__ float vec_elem(const void* p, int dt, int64_t i) {
-  return dt == F32 ? __ldg(static_cast<const float*>(p) + i) : dev::load_elem<DT>(p, uint64_t(i));
+__device__ __forceinline__ float get(const void* p, int64_t i) {
+  if constexpr (DT == F32) return __ldg(static_cast<const float*>(p) + i);
+  const uint16_t v = __ldg(static_cast<const uint16_t*>(p) + i);
+  return DT == BF16 ? __uint_as_float(uint32_t(v) << 16) : __half2float(__ushort_as_half(v));
+}
+template <int DT>
+__device__ __forceinline__ void put(void* p, int64_t i, float v) {
+  if constexpr (DT == F32) static_cast<float*>(p)[i] = v;
+  else if constexpr (DT == BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// Sum over the CTA; `slot` alternates between consecutive calls, so one
-// barrier per call keeps a call's partials apart from the next one's.
-__device__ __forceinline__ float cta_sum(float v, float* part, int& slot) {
+// Sum over the CTA's `threads` (blockDim.x, at most 1024); `slot` alternates
+// between consecutive calls, so one barrier per call keeps a call's partials
+// apart from the next one's.  Every thread adds the warps' partials itself:
+// their few broadcast reads are shorter than a second round of shuffles.
+__device__ __forceinline__ float cta_sum(float v, float4* part, int& slot) {
   const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5, warps = int(blockDim.x) >> 5;
 #pragma unroll
   for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
   if (warps == 1) return v;
-  float* p = part + 32 * slot;
+  float4* p = part + 8 * slot;
   slot ^= 1;
-  if (lane == 0) p[warp] = v;
+  if (lane == 0) reinterpret_cast<float*>(p)[warp] = v;
+  // the last warp clears what the last float4 has behind the partials
+  if (warp == warps - 1 && lane > 0 && warp + lane < ((warps + 3) & ~3)) reinterpret_cast<float*>(p)[warp + lane] = 0.0f;
   __syncthreads();
-  v = lane < warps ? p[lane] : 0.0f;
-#pragma unroll
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
-  return v;
+  float4 s = p[0];
+  for (int k = 1; 4 * k < warps; ++k) {
+    const float4 u = p[k];
+    s.x += u.x, s.y += u.y, s.z += u.z, s.w += u.w;
+  }
+  return (s.x + s.y) + (s.z + s.w);
 }
 
 // 1 / sqrt of the mean square of v over `dim` values (layer: after taking the
 // mean off v).  N values per thread, absent ones 0 and not counted.
 template <int N>
-__device__ __forceinline__ float normalise(float (&v)[N], int n, float inv_dim, float eps, int kind, float* part,
+__device__ __forceinline__ float normalise(float (&v)[N], int n, float inv_dim, float eps, int kind, float4* part,
                                            int& slot) {
   if (kind == NORM_LAYER) {
     float s = 0.0f;
@@ -58,24 +78,42 @@ __device__ __forceinline__ float normalise(float (&v)[N], int n, float inv_dim, 
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = j < n ? v[j] - mean : 0.0f;
   }
-  float q = 0.0f;
+  // two running sums in one packed register pair
+  static_assert(N % 2 == 0, "");
+  float2 q2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-  for (int j = 0; j < N; ++j) q = fmaf(v[j], v[j], q);
-  return 1.0f / sqrtf(cta_sum(q, part, slot) * inv_dim + eps);
+  for (int j = 0; j < N; j += 2) {
+    const float2 p = make_float2(v[j], v[j + 1]);
+    q2 = __ffma2_rn(p, p, q2);
+  }
+  const float q = q2.x + q2.y;
+  return rsqrtf(fmaf(cta_sum(q, part, slot), inv_dim, eps));
 }
 
 template <int DT>
-__device__ __forceinline__ void load_row8(const void* base, int64_t elem, float* x) {
-  if constexpr (DT == F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + elem);
-    const float4 a = p[0], b = p[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const uint4 r = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + elem);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+struct Raw8 {  // 8 values as loaded
+  uint4 w[DT == F32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_row8(const void* base, int64_t elem) {
+  Raw8<DT> r;
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(base) + elem * (DT == F32 ? 4 : 2));
+#pragma unroll
+  for (int k = 0; k < (DT == F32 ? 2 : 1); ++k) r.w[k] = p[k];
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack_row8(const Raw8<DT>& r, float* x) {
+#pragma unroll
+  for (int k = 0; k < (DT == F32 ? 2 : 1); ++k) {
+    const uint32_t w[4] = {r.w[k].x, r.w[k].y, r.w[k].z, r.w[k].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if constexpr (DT == BF16) {
+      if constexpr (DT == F32) {
+        x[4 * k + j] = __uint_as_float(w[j]);
+      } else if constexpr (DT == BF16) {
         x[2 * j] = __uint_as_float(w[j] << 16);
         x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
       } else {
@@ -103,6 +141,13 @@ __device__ __forceinline__ void store_row8(void* base, int64_t elem, const float
   }
 }
 
+// 8 consecutive elements of such a vector, 16-byte aligned.
+template <int DT>
+__device__ __forceinline__ void vec8(const void* p, int dt, int64_t i, float* x) {
+  if (dt == F32) unpack_row8<F32>(load_row8<F32>(p, i), x);
+  else unpack_row8<DT>(load_row8<DT>(p, i), x);
+}
+
 // The modulation group of row t: -1 when its index is outside the rows there
 // are (such a row is filled with NaN: an index is device data, which the host
 // cannot check, and a row computed with another group's vectors would pass
@@ -113,164 +158,254 @@ __device__ __forceinline__ int group_of(const ResidualNormParams& a, uint64_t t)
   return g >= 0 && g < a.mod_rows ? g : -1;
 }
 
-// dim a multiple of 8 with 16-byte aligned rows: thread j of the CTA owns the
-// 8-value chunks j, j + threads, ... (V of them).
-template <int DT, int V>
-__global__ void __launch_bounds__(1024) k_residual_norm_vec(const ResidualNormParams a) {
-  __shared__ float part[64];
+// The products of group g (-1: NaN) for the 8 columns from i on.
+template <int DT>
+__device__ __forceinline__ void products8(const ResidualNormParams& a, int g, int64_t i, float* G, float* W, float* S) {
+  const int64_t m = int64_t(max(g, 0)) * a.dim + i;
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) G[j] = W[j] = 1.0f, S[j] = 0.0f;
+  if (a.gate) vec8<DT>(a.gate, a.mod_dtype, m, G);
+  if (a.shift) vec8<DT>(a.shift, a.mod_dtype, m, S);
+  if (a.weight) vec8<DT>(a.weight, a.weight_dtype, i, W);
+  if (a.post_weight) {
+    vec8<DT>(a.post_weight, a.weight_dtype, i, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) G[j] *= v[j];
+  }
+  if (a.scale) {
+    vec8<DT>(a.scale, a.mod_dtype, m, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) W[j] *= 1.0f + v[j];
+  }
+  if (g < 0) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) G[j] = W[j] = S[j] = __int_as_float(0x7FFFFFFF);
+  }
+}
+
+// dim a multiple of 8 up to 8192, everything 16-byte aligned: thread j of the
+// CTA owns the 8-column chunks j and j + threads, and in shared memory the
+// bytes of its chunks of the kAhead rows on their way.
+template <int DT, int kAhead>
+__global__ void __maxnreg__(96) k_residual_norm_vec(const ResidualNormParams a) {
+  extern __shared__ uint4 ring[];
+  __shared__ float4 part[16];
   int slot = 0;
-  const int tid = int(threadIdx.x), threads = int(blockDim.x);
-  const int chunks = int(a.dim / 8);
+  constexpr int kSize = DT == F32 ? 4 : 2, kPieces = DT == F32 ? 2 : 1;  // 16-byte pieces per chunk
+  const int threads = int(blockDim.x), chunks = int(a.dim / 8);
+  const int c0 = int(threadIdx.x);
+  const bool have[2] = {c0 < chunks, c0 + threads < chunks};
+  const int n = 8 * (int(have[0]) + int(have[1]));  // values this thread holds
   const float inv_dim = 1.0f / float(a.dim);
   const uint64_t r0 = uint64_t(blockIdx.x) * a.rows_per_cta;
-  const uint64_t r1 = min(a.tokens, r0 + a.rows_per_cta);
-  // the group's vectors
-  float G[8 * V], W[8 * V], S[8 * V];
-  int group = -2;
-  int n = 0;  // values this thread holds
+  const int rows = int(min(a.tokens - r0, a.rows_per_cta));
+  // piece p of chunk k of x (0) or branch (1) in ring row `row`
+  auto piece = [&](int row, int tensor, int k, int p) {
+    return ring + ((row * 2 + tensor) * kPieces + p) * chunks + c0 + k * threads;
+  };
+  auto request = [&](int r, int row) {
+    if (r < rows) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) n += tid + k * threads < chunks ? 8 : 0;
-  for (uint64_t t = r0; t < r1; ++t) {
-    const int g = group_of(a, t);
-    float h[8 * V], b[8 * V];
+      for (int tensor = 0; tensor < 2; ++tensor) {
+        const void* src = tensor ? a.branch : a.x;
+        if (!src) continue;
+        const unsigned char* q = static_cast<const unsigned char*>(src) +
+                                 ((int64_t(r0) + r) * (tensor ? a.branch_stride : a.x_stride) + 8 * c0) * kSize;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const int c = tid + k * threads;
-      if (c < chunks) {
-        load_row8<DT>(a.x, int64_t(t) * a.x_stride + 8 * c, h + 8 * k);
-        if (a.branch) load_row8<DT>(a.branch, int64_t(t) * a.branch_stride + 8 * c, b + 8 * k);
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p)
+            if (have[k])
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
+                               __cvta_generic_to_shared(piece(row, tensor, k, p)))),
+                           "l"(q + 8 * k * threads * kSize + 16 * p)
+                           : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto arrived = [&](int row, int tensor, int k, float* x) {
+    Raw8<DT> raw;
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) raw.w[p] = *piece(row, tensor, k, p);
+    unpack_row8<DT>(raw, x);
+  };
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) request(d, d);
+  int next_group = group_of(a, r0), group = -2, row = 0;
+  float G[16], W[16], S[16];
+  for (int r = 0; r < rows; ++r) {
+    const int g = next_group;
+    if (r + 1 < rows) next_group = group_of(a, r0 + uint64_t(r) + 1);
+    if (g != group) {
+      group = g;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (have[k]) products8<DT>(a, g, 8 * int64_t(c0 + k * threads), G + 8 * k, W + 8 * k, S + 8 * k);
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+    float h[16], b[16];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (have[k]) {
+        arrived(row, 0, k, h + 8 * k);
+        if (a.branch) arrived(row, 1, k, b + 8 * k);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) h[8 * k + j] = b[8 * k + j] = 0.0f;
       }
     }
-    if (g != group) {
-      group = g;
+    request(r + kAhead, row);
+    if (++row == kAhead) row = 0;
+    // v = v * inv * P + Q on packed pairs
+    auto scaled = [](const float* v, float inv, const float* P, const float* Q, float* out) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = tid + k * threads;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float gg = 1.0f, ww = 1.0f, ss = 0.0f;
-          if (c < chunks) {
-            const int64_t i = 8 * int64_t(c) + j, m = int64_t(max(g, 0)) * a.dim + i;
-            if (a.gate) gg = vec_elem<DT>(a.gate, a.mod_dtype, m);
-            if (a.post_weight) gg *= vec_elem<DT>(a.post_weight, a.weight_dtype, i);
-            if (a.weight) ww = vec_elem<DT>(a.weight, a.weight_dtype, i);
-            if (a.scale) ww *= 1.0f + vec_elem<DT>(a.scale, a.mod_dtype, m);
-            if (a.shift) ss = vec_elem<DT>(a.shift, a.mod_dtype, m);
-          }
-          if (g < 0) gg = ww = ss = __int_as_float(0x7FFFFFFF);
-          G[8 * k + j] = gg;
-          W[8 * k + j] = ww;
-          S[8 * k + j] = ss;
-        }
+      for (int j = 0; j < 8; j += 2) {
+        const float2 u = __ffma2_rn(__fmul2_rn(make_float2(v[j], v[j + 1]), make_float2(inv, inv)),
+                                    make_float2(P[j], P[j + 1]), make_float2(Q[j], Q[j + 1]));
+        out[j] = u.x, out[j + 1] = u.y;
       }
-    }
+    };
+    const int64_t t = int64_t(r0) + r;
     if (a.branch) {
-      float inv = 1.0f;
-      if (a.post) inv = normalise(b, n, inv_dim, a.eps, a.post, part, slot);
+      const float inv = a.post ? normalise(b, n, inv_dim, a.eps, a.post, part, slot) : 1.0f;
 #pragma unroll
-      for (int j = 0; j < 8 * V; ++j) h[j] = fmaf(b[j] * inv, G[j], h[j]);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = tid + k * threads;
-        if (c < chunks && a.h_out) store_row8<DT>(a.h_out, int64_t(t) * a.h_stride + 8 * c, h + 8 * k);
+      for (int k = 0; k < 2; ++k) {
+        if (!have[k]) continue;
+        scaled(b + 8 * k, inv, G + 8 * k, h + 8 * k, h + 8 * k);
+        store_row8<DT>(a.h_out, t * a.h_stride + 8 * (c0 + k * threads), h + 8 * k);
       }
     }
     if (a.norm) {
       const float inv = normalise(h, n, inv_dim, a.eps, a.norm, part, slot);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int c = tid + k * threads;
-        if (c < chunks) {
-          float y[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = fmaf(h[8 * k + j] * inv, W[8 * k + j], S[8 * k + j]);
-          store_row8<DT>(a.y_out, int64_t(t) * a.y_stride + 8 * c, y);
-        }
+      for (int k = 0; k < 2; ++k) {
+        if (!have[k]) continue;
+        float y[8];
+        scaled(h + 8 * k, inv, W + 8 * k, S + 8 * k, y);
+        store_row8<DT>(a.y_out, t * a.y_stride + 8 * (c0 + k * threads), y);
       }
     }
   }
 }
 
-// Any dim up to kResidualNormMaxDim and any alignment: one CTA per row, the
-// row's f32 values in shared memory (each thread touches only its own).
-template <int DT>
-__global__ void __launch_bounds__(512) k_residual_norm_any(const ResidualNormParams a) {
-  extern __shared__ float row[];
-  __shared__ float part[64];
+// The n values tid, tid + threads, ... of a row from element `base` on, others 0.
+template <int DT, int E>
+__device__ __forceinline__ void get_row(const void* p, int64_t base, int n, int threads, float (&v)[E]) {
+  const int64_t at = base + int64_t(threadIdx.x);
+#pragma unroll
+  for (int k = 0; k < E; ++k) v[k] = k < n ? get<DT>(p, at + k * threads) : 0.0f;
+}
+// The same of a vector that is f32 or the stream's type.
+template <int DT, int E>
+__device__ __forceinline__ void get_vec(const void* p, int dt, int64_t base, int n, int threads, float (&v)[E]) {
+  if (dt == F32) get_row<F32>(p, base, n, threads, v);
+  else get_row<DT>(p, base, n, threads, v);
+}
+template <int DT, int E>
+__device__ __forceinline__ void put_row(void* p, int64_t base, int n, int threads, const float (&v)[E]) {
+  const int64_t at = base + int64_t(threadIdx.x);
+#pragma unroll
+  for (int k = 0; k < E; ++k)
+    if (k < n) put<DT>(p, at + k * threads, v[k]);
+}
+
+// Any dim and any alignment: blockDim.x threads per row, each holding the E
+// values tid, tid + blockDim.x, ...; one row per CTA, or one per warp when 32
+// threads suffice.
+template <int DT, int E, int kMaxThreads>
+__global__ void __launch_bounds__(kMaxThreads) k_residual_norm_any(const ResidualNormParams a) {
+  __shared__ float4 part[16];
   int slot = 0;
   const int tid = int(threadIdx.x), threads = int(blockDim.x), dim = int(a.dim);
+  const uint64_t t = uint64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (t >= a.tokens) return;  // only where a row is a warp: no barrier is skipped
   const float inv_dim = 1.0f / float(dim), nan = __int_as_float(0x7FFFFFFF);
-  const uint64_t t = blockIdx.x;
+  const int n = tid < dim ? (dim - tid + threads - 1) / threads : 0;
+  float h[E], v[E];
+  get_row<DT>(a.x, int64_t(t) * a.x_stride, n, threads, h);
   const int g = group_of(a, t);
   const int64_t mrow = int64_t(max(g, 0)) * a.dim;
-  auto norm_of = [&](int kind, float& mean) {
-    mean = 0.0f;
-    if (kind == NORM_LAYER) {
-      float s = 0.0f;
-      for (int i = tid; i < dim; i += threads) s += row[i];
-      mean = cta_sum(s, part, slot) * inv_dim;
-    }
-    float q = 0.0f;
-    for (int i = tid; i < dim; i += threads) q = fmaf(row[i] - mean, row[i] - mean, q);
-    return 1.0f / sqrtf(cta_sum(q, part, slot) * inv_dim + a.eps);
-  };
-  float mean = 0.0f, inv = 1.0f;
   if (a.branch) {
-    if (a.post) {
-      for (int i = tid; i < dim; i += threads)
-        row[i] = dev::load_elem<DT>(a.branch, uint64_t(int64_t(t) * a.branch_stride + i));
-      inv = norm_of(a.post, mean);
+    get_row<DT>(a.branch, int64_t(t) * a.branch_stride, n, threads, v);
+    const float inv = a.post ? normalise(v, n, inv_dim, a.eps, a.post, part, slot) : 1.0f;
+    const float one = g < 0 ? nan : inv;
+#pragma unroll
+    for (int k = 0; k < E; ++k) v[k] *= one;
+    float w[E];
+    if (a.post_weight) {
+      get_vec<DT>(a.post_weight, a.weight_dtype, 0, n, threads, w);
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] *= w[k];
     }
-    for (int i = tid; i < dim; i += threads) {
-      const float b = a.post ? row[i] : dev::load_elem<DT>(a.branch, uint64_t(int64_t(t) * a.branch_stride + i));
-      float gg = a.gate ? vec_elem<DT>(a.gate, a.mod_dtype, mrow + i) : 1.0f;
-      if (a.post_weight) gg *= vec_elem<DT>(a.post_weight, a.weight_dtype, i);
-      if (g < 0) gg = nan;
-      const float h =
-          fmaf((b - mean) * inv, gg, dev::load_elem<DT>(a.x, uint64_t(int64_t(t) * a.x_stride + i)));
-      row[i] = h;
-      if (a.h_out) dev::store_elem<DT>(a.h_out, uint64_t(int64_t(t) * a.h_stride + i), h);
+    if (a.gate) {
+      get_vec<DT>(a.gate, a.mod_dtype, mrow, n, threads, w);
+#pragma unroll
+      for (int k = 0; k < E; ++k) v[k] *= w[k];
     }
-  } else {
-    for (int i = tid; i < dim; i += threads)
-      row[i] = dev::load_elem<DT>(a.x, uint64_t(int64_t(t) * a.x_stride + i));
+#pragma unroll
+    for (int k = 0; k < E; ++k) h[k] += v[k];
+    put_row<DT>(a.h_out, int64_t(t) * a.h_stride, n, threads, h);
   }
   if (!a.norm) return;
-  inv = norm_of(a.norm, mean);
-  for (int i = tid; i < dim; i += threads) {
-    float ww = a.weight ? vec_elem<DT>(a.weight, a.weight_dtype, i) : 1.0f;
-    if (a.scale) ww *= 1.0f + vec_elem<DT>(a.scale, a.mod_dtype, mrow + i);
-    float ss = a.shift ? vec_elem<DT>(a.shift, a.mod_dtype, mrow + i) : 0.0f;
-    if (g < 0) ww = ss = nan;
-    dev::store_elem<DT>(a.y_out, uint64_t(int64_t(t) * a.y_stride + i), fmaf((row[i] - mean) * inv, ww, ss));
+  const float inv = normalise(h, n, inv_dim, a.eps, a.norm, part, slot);
+  const float one = g < 0 ? nan : inv;
+#pragma unroll
+  for (int k = 0; k < E; ++k) h[k] *= one;
+  if (a.weight) {
+    get_vec<DT>(a.weight, a.weight_dtype, 0, n, threads, v);
+#pragma unroll
+    for (int k = 0; k < E; ++k) h[k] *= v[k];
   }
+  if (a.scale) {
+    get_vec<DT>(a.scale, a.mod_dtype, mrow, n, threads, v);
+#pragma unroll
+    for (int k = 0; k < E; ++k) h[k] = fmaf(h[k], v[k], h[k]);
+  }
+  if (a.shift) {
+    get_vec<DT>(a.shift, a.mod_dtype, mrow, n, threads, v);
+#pragma unroll
+    for (int k = 0; k < E; ++k) h[k] += v[k];
+  }
+  put_row<DT>(a.y_out, int64_t(t) * a.y_stride, n, threads, h);
+}
+
+template <int DT, int kAhead>
+cudaError_t launch_vec(ResidualNormParams a, size_t row, cudaStream_t s) {
+  const int64_t chunks = a.dim / 8;
+  const int threads = int(((chunks + 1) / 2 + 31) / 32 * 32);
+  // as many CTAs as 96 registers a thread and the rings let an SM hold
+  const size_t smem = row * kAhead;
+  const uint64_t per_sm = std::max<uint64_t>(1, std::min<uint64_t>({640u / uint64_t(threads), 220 * 1024 / (smem + 1280), 12}));
+  a.rows_per_cta = (a.tokens + per_sm * 148 - 1) / (per_sm * 148);
+  const unsigned grid = unsigned((a.tokens + a.rows_per_cta - 1) / a.rows_per_cta);
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(k_residual_norm_vec<DT, kAhead>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+    if (e != cudaSuccess) return e;
+  }
+  k_residual_norm_vec<DT, kAhead><<<grid, threads, smem, s>>>(a);
+  return cudaGetLastError();
+}
+
+// x and branch of a row in the ring: four rows where two CTAs' rings then fit
+// an SM, else two (of at most 64 KB).
+template <int DT>
+cudaError_t launch_vec(const ResidualNormParams& a, cudaStream_t s) {
+  const size_t row = size_t(a.dim) * 2 * dtype_size(DT);
+  return row * 4 <= 100 * 1024 ? launch_vec<DT, 4>(a, row, s) : launch_vec<DT, 2>(a, row, s);
 }
 
 template <int DT>
-cudaError_t launch_dt(ResidualNormParams a, bool vec, cudaStream_t s) {
-  if (vec) {
-    const int chunks = int(a.dim / 8);
-    const int v = chunks <= 1024 ? 1 : 2;
-    const int threads = ((chunks + v - 1) / v + 31) / 32 * 32;
-    // runs of consecutive rows, about four CTAs of 256 threads' worth per SM
-    const uint64_t want = uint64_t(148) * uint64_t(threads >= 1024 ? 1 : 1024 / threads);
-    a.rows_per_cta = (a.tokens + want - 1) / want;
-    const unsigned grid = unsigned((a.tokens + a.rows_per_cta - 1) / a.rows_per_cta);
-    if (v == 1) k_residual_norm_vec<DT, 1><<<grid, threads, 0, s>>>(a);
-    else k_residual_norm_vec<DT, 2><<<grid, threads, 0, s>>>(a);
-  } else {
-    const int threads = a.dim <= 1024 ? 128 : a.dim <= 4096 ? 256 : 512;
-    const size_t smem = size_t(a.dim) * sizeof(float);
-    if (smem > 40 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(k_residual_norm_any<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 int(kResidualNormMaxDim * sizeof(float)));
-      if (e != cudaSuccess) return e;
-    }
-    k_residual_norm_any<DT><<<unsigned(a.tokens), threads, smem, s>>>(a);
-  }
+cudaError_t launch_any(const ResidualNormParams& a, cudaStream_t s) {
+  const int per = a.dim <= 2048 ? 8 : 16;
+  const int threads = a.dim <= 16384 ? int((a.dim + 32 * per - 1) / (32 * per) * 32) : 1024;
+  const dim3 block(threads, threads == 32 ? 4 : 1);
+  const unsigned grid = unsigned((a.tokens + block.y - 1) / block.y);
+  if (per == 8) k_residual_norm_any<DT, 8, 256><<<grid, block, 0, s>>>(a);
+  else if (a.dim <= 16384) k_residual_norm_any<DT, 16, 1024><<<grid, block, 0, s>>>(a);
+  else k_residual_norm_any<DT, 32, 1024><<<grid, block, 0, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -279,14 +414,15 @@ cudaError_t launch_dt(ResidualNormParams a, bool vec, cudaStream_t s) {
 cudaError_t launch_residual_norm(const ResidualNormParams& a, int dtype, cudaStream_t s) {
   if (a.tokens == 0) return cudaSuccess;
   const size_t es = dtype_size(dtype);
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.branch) |
-                         reinterpret_cast<uintptr_t>(a.h_out) | reinterpret_cast<uintptr_t>(a.y_out) |
-                         uintptr_t((a.x_stride | a.branch_stride | a.h_stride | a.y_stride) * int64_t(es));
-  const bool vec = a.dim % 8 == 0 && a.dim <= 16384 && (bits & 15u) == 0;
+  uintptr_t bits = uintptr_t((a.x_stride | a.branch_stride | a.h_stride | a.y_stride) * int64_t(es));
+  for (const void* p : {a.x, a.branch, static_cast<const void*>(a.h_out), static_cast<const void*>(a.y_out),
+                        a.post_weight, a.weight, a.gate, a.scale, a.shift})
+    bits |= reinterpret_cast<uintptr_t>(p);
+  const bool vec = a.dim % 8 == 0 && a.dim <= 8192 && (bits & 15u) == 0;
   switch (dtype) {
-    case F32: return launch_dt<F32>(a, vec, s);
-    case BF16: return launch_dt<BF16>(a, vec, s);
-    default: return launch_dt<F16>(a, vec, s);
+    case F32: return vec ? launch_vec<F32>(a, s) : launch_any<F32>(a, s);
+    case BF16: return vec ? launch_vec<BF16>(a, s) : launch_any<BF16>(a, s);
+    default: return vec ? launch_vec<F16>(a, s) : launch_any<F16>(a, s);
   }
 }
 

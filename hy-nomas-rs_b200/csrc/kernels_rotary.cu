@@ -17,8 +17,11 @@
 // as well, as the reference does between its two modules).
 //
 // Both kernels move bytes: each value is read and written once.  A token's
-// D/2 angles serve all its heads, so a CTA computes them once into shared
-// memory for a few tokens and then streams those tokens' rows.
+// D / 2 angles serve all its heads: a group of lanes computes one token's
+// angles, each lane those of its own columns, into registers and then streams
+// that token's heads, several rows ahead.
+#include <type_traits>
+
 #include "nkv_device.cuh"
 #include "nkv_kernels.h"
 
@@ -28,17 +31,27 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kRotMaxPairs = kRotaryMaxDim / 2;
 
-// cos and sin of an f64 angle, rounded to f32.  The quadrant reduction (three
-// parts of pi/2: the product n * P1 is exact inside the fma, what P1 lacks is
-// added by P2 and P3) leaves |r| <= pi/4, where the f32 functions are within
-// 2 ulp.
+// cos and sin of an f64 angle in f32.  The quadrant reduction in f64 (two parts
+// of pi / 2; the product with the first is exact inside the fma) leaves |r| <=
+// pi / 4, where the Taylor sums sin r = r - r^3/3! + ... + r^9/9! and cos r = 1
+// - r^2/2! + ... + r^10/10! stop below 2^-29 of 1 and each last rounding is one
+// of f32.  Their few multiply-adds replace library calls whose argument
+// reduction this kernel has no use for.
 __device__ __forceinline__ float2 cos_sin(double a) {
   const double n = rint(a * 0.63661977236758134308);  // 2 / pi
   double r = fma(-n, 1.5707963267948965580, a);       // pi / 2 rounded to 53 bits
   r = fma(-n, 6.1232339957367660359e-17, r);          // the next 53 bits
   const int q = int(__double2ll_rn(n)) & 3;
-  float s, c;
-  sincosf(float(r), &s, &c);
+  const float x = float(r), y = x * x;
+  float s = fmaf(2.7557319e-6f, y, -1.9841270e-4f);  // 1/9!, -1/7!
+  s = fmaf(s, y, 8.3333333e-3f);                      // 1/5!
+  s = fmaf(s, y, -1.6666667e-1f);                     // -1/3!
+  s = fmaf(s * y, x, x);
+  float c = fmaf(-2.7557319e-7f, y, 2.4801587e-5f);  // -1/10!, 1/8!
+  c = fmaf(c, y, -1.3888889e-3f);                     // -1/6!
+  c = fmaf(c, y, 4.1666667e-2f);                      // 1/4!
+  c = fmaf(c, y, -0.5f);
+  c = fmaf(c, y, 1.0f);
   if (q & 1) {
     const float t = s;
     s = c;
@@ -58,17 +71,35 @@ __device__ __forceinline__ double position(const RopePositions& P, uint64_t t, i
   return double(__ldg(static_cast<const float*>(P.data) + i));
 }
 
-__global__ void __launch_bounds__(kRotThreads) k_rope_tables(const RopePositions P, uint64_t tokens, float* cos_out,
-                                                             float* sin_out) {
-  const uint64_t total = tokens * uint64_t(P.pairs);
-  for (uint64_t i = blockIdx.x * uint64_t(kRotThreads) + threadIdx.x; i < total;
-       i += uint64_t(gridDim.x) * kRotThreads) {
-    const uint64_t t = i / uint64_t(P.pairs);
-    const int p = int(i - t * uint64_t(P.pairs));
-    const float2 cs = cos_sin(position(P, t, P.axis[p]) * P.freq[p]);
+// Calls f(token, pair, cos, sin) for the CTA's tokens t0 .. t0 + nt.  A thread
+// keeps its pairs p, p + blockDim.x, ... over all its tokens: the frequencies
+// lie in the kernel's parameters, where lanes that index differently are
+// served one at a time, so each is read once per thread.
+template <typename F>
+__device__ __forceinline__ void for_angles(const RopePositions& P, uint64_t t0, int nt, F&& f) {
+  const int lanes = min(P.pairs, int(blockDim.x));      // threads along the pairs
+  const int rows = int(blockDim.x) / lanes;             // tokens at a time
+  const int row = int(threadIdx.x) / lanes;
+  if (row >= rows) return;
+  for (int p = int(threadIdx.x) - row * lanes; p < P.pairs; p += lanes) {
+    const double freq = P.freq[p];
+    const int axis = P.axis[p];
+    for (int t = row; t < nt; t += rows) {
+      const float2 cs = cos_sin(position(P, t0 + uint64_t(t), axis) * freq);
+      f(t, p, cs);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kRotThreads) k_rope_tables(const RopePositions P, uint64_t tokens, int per_cta,
+                                                             float* cos_out, float* sin_out) {
+  const uint64_t t0 = uint64_t(blockIdx.x) * uint64_t(per_cta);
+  const int nt = int(min(uint64_t(per_cta), tokens - t0));
+  for_angles(P, t0, nt, [&](int t, int p, float2 cs) {
+    const uint64_t i = (t0 + uint64_t(t)) * uint64_t(P.pairs) + uint64_t(p);
     cos_out[i] = cs.x;
     sin_out[i] = cs.y;
-  }
+  });
 }
 
 template <int DT>
@@ -135,110 +166,183 @@ __device__ __forceinline__ void store_chunk(void* base, int64_t elem, const floa
   }
 }
 
-// The angles of this CTA's tokens as (cos, sin) pairs [token][pair].
-__device__ __forceinline__ void fill_angles(const RopePositions& P, float2* table, uint64_t t0, int nt) {
-  for (int i = threadIdx.x; i < nt * P.pairs; i += blockDim.x) {
-    const int t = i / P.pairs, p = i - t * P.pairs;
-    table[i] = cos_sin(position(P, t0 + uint64_t(t), P.axis[p]) * P.freq[p]);
-  }
-}
-
 // head_dim 16 * LPR, 16-byte aligned rows: LPR lanes per (token, head), each
-// two 16-byte (f32: 32-byte) chunks.  Interleaved pairs: chunks 2l, 2l + 1.
+// two chunks of 8 values; consecutive lanes take consecutive chunks, so an
+// access covers whole lines.  Interleaved pairs: chunks l and l + LPR.
 // Half-split pairs: chunk l of the first and of the second half of the rotated
 // values, so both members of a pair meet in one thread; lanes past R / 16 take
 // two chunks of the values that pass through (R is a multiple of 16).
+// 2^log_hp such groups share a token's heads, where one group per token would
+// leave the GPU empty; each computes the angles again.
 template <int DT, int LPR>
-__global__ void __launch_bounds__(kRotThreads) k_rotary_vec(const RotaryParams a) {
-  extern __shared__ float2 table[];
+__global__ void __launch_bounds__(kRotThreads, 3) k_rotary_vec(const RotaryParams a) {
   constexpr int D = 16 * LPR;
+  // rows a thread has in flight, by cp.async into its own bytes of shared memory
+  constexpr int kAhead = DT == F32 ? 2 : 4, kPieces = DT == F32 ? 2 : 1;  // 16-byte pieces per chunk
+  __shared__ uint4 ring[kAhead][2][kPieces][kRotThreads];
   const RopePositions& P = a.pos;
-  const uint64_t t0 = uint64_t(blockIdx.x) * uint64_t(a.tokens_per_cta);
-  const int nt = int(min(uint64_t(a.tokens_per_cta), a.tokens - t0));
-  fill_angles(P, table, t0, nt);
-  __syncthreads();
-  const int l = int(threadIdx.x) % LPR, slot = int(threadIdx.x) / LPR;
-  constexpr int kSlots = kRotThreads / LPR;
-  const int R = 2 * P.pairs, heads = a.side[0].heads + a.side[1].heads;
-  int c0 = 2 * l, c1 = 2 * l + 1;
-  int n_rot;  // pairs this thread rotates
-  int p0;     // its first pair
+  __shared__ double freq[D / 2];
+  __shared__ uint8_t axis[D / 2];
+  const int l = int(threadIdx.x) % LPR;
+  const uint64_t group = (uint64_t(blockIdx.x) * kRotThreads + threadIdx.x) / LPR;
+  const int hp = 1 << a.log_hp, h0 = int(group) & (hp - 1);
+  const uint64_t t = group >> a.log_hp;
+  const bool live = t < a.tokens;
+  const int R = 2 * P.pairs, q_heads = a.side[0].heads, heads = q_heads + a.side[1].heads;
+  int c0 = l, c1 = l + LPR;
+  int n_rot0 = 0, n_rot1 = 0;  // rotated pairs of the chunks (half-split: of both together, in n_rot0)
   if (a.interleaved) {
-    p0 = 8 * l;
-    n_rot = max(0, min(8, P.pairs - p0));
+    n_rot0 = max(0, min(4, P.pairs - 4 * c0));
+    n_rot1 = max(0, min(4, P.pairs - 4 * c1));
   } else if (l < R / 16) {
-    c0 = l;
     c1 = l + R / 16;
-    p0 = 8 * l;
-    n_rot = 8;
+    n_rot0 = 8;
   } else {
-    c0 = R / 8 + 2 * (l - R / 16);
-    c1 = c0 + 1;
-    p0 = 0;
-    n_rot = 0;
+    c0 = R / 8 + (l - R / 16);
+    c1 = c0 + (D - R) / 16;
   }
-  const int rows = nt * heads, rounds = (rows + kSlots - 1) / kSlots;
-  for (int it = 0; it < rounds; ++it) {
-    const int row = it * kSlots + slot;
-    const bool have = row < rows;  // every lane stays for the shuffles
-    const int t = have ? row / heads : 0;
-    int h = have ? row - t * heads : 0;
-    const int sd = h >= a.side[0].heads ? 1 : 0;
-    const RotarySide& S = a.side[sd];
-    if (sd) h -= a.side[0].heads;
-    float x[16];
-    if (have) {
-      const int64_t base = int64_t(t0 + uint64_t(t)) * S.in_token + int64_t(h) * S.in_head;
-      const Chunk<DT> u = load_chunk<DT>(S.in, base + 8 * c0), v = load_chunk<DT>(S.in, base + 8 * c1);
-      unpack<DT>(u, x);
-      unpack<DT>(v, x + 8);
-    } else {
+  constexpr int kSize = DT == F32 ? 4 : 2;
+  const unsigned char* in_q = static_cast<const unsigned char*>(a.side[0].in) + int64_t(t) * a.side[0].in_token * kSize;
+  const unsigned char* in_k = static_cast<const unsigned char*>(a.side[1].in) + int64_t(t) * a.side[1].in_token * kSize;
+  auto request = [&](int b, int h) {
+    if (live && h < heads) {
+      const unsigned char* row = h < q_heads ? in_q + int64_t(h) * a.side[0].in_head * kSize
+                                             : in_k + int64_t(h - q_heads) * a.side[1].in_head * kSize;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
+                           __cvta_generic_to_shared(&ring[b][k][p][threadIdx.x]))),
+                       "l"(row + 8 * (k ? c1 : c0) * kSize + 16 * p)
+                       : "memory");
     }
-    if (a.norm) {
-      float s[2] = {0.0f, 0.0f};
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto arrived = [&](int b, int k, float* x) {
+    Chunk<DT> c;
+    c.a = *reinterpret_cast<const decltype(c.a)*>(&ring[b][k][0][threadIdx.x]);
+    if constexpr (DT == F32) c.b = *reinterpret_cast<const float4*>(&ring[b][k][kPieces - 1][threadIdx.x]);
+    unpack<DT>(c, x);
+  };
+  // the first rows are on their way while the angles are computed
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[j & 1] = fmaf(x[j], x[j], s[j & 1]);
-      float ss = s[0] + s[1];
+  for (int b = 0; b < kAhead; ++b) request(b, h0 + b * hp);
+  // (the parameters serve lanes that index differently one at a time)
+  if (threadIdx.x < P.pairs) {
+    freq[threadIdx.x] = P.freq[threadIdx.x];
+    axis[threadIdx.x] = P.axis[threadIdx.x];
+  }
+  __syncthreads();
+  // Pair j of this thread is (x[ia(j)], x[ib(j)]) of its 16 values: with the
+  // gains w folded in,
+  //   a' = a (w_a c) - b (w_b s),  b' = b (w_b c) + a (w_a s),
+  // on two pairs at a time.  A pair that passes through is only multiplied by
+  // its gains (a sine of 0 would turn an infinite partner into a NaN).
+  auto ia = [&](int j, bool inter) { return inter ? 2 * j : j; };
+  auto ib = [&](int j, bool inter) { return inter ? 2 * j + 1 : 8 + j; };
+  float2 cs[8];
+  uint32_t rotates = 0;  // one bit per pair
+  {
+    const int pa = a.interleaved ? 4 * c0 : 8 * c0, pb = a.interleaved ? 4 * c1 : 8 * c0 + 4;
+    const int na = a.interleaved ? n_rot0 : n_rot0 / 2, nb = a.interleaved ? n_rot1 : n_rot0 / 2;
 #pragma unroll
-      for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
-      const float inv = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-      if (S.weight) {
-        float w[16];
-        unpack<DT>(load_chunk<DT>(S.weight, 8 * c0), w);
-        unpack<DT>(load_chunk<DT>(S.weight, 8 * c1), w + 8);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] *= inv * w[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] *= inv;
+    for (int j = 0; j < 8; ++j) {
+      const int p = j < 4 ? pa + j : pb + j - 4;
+      cs[j] = make_float2(1.0f, 0.0f);
+      if (j < 4 ? j < na : j - 4 < nb) {
+        rotates |= 1u << j;
+        if (live) cs[j] = cos_sin(position(P, t, axis[p]) * freq[p]);
       }
     }
-    if (!have) continue;
-    const float2* cs = table + t * P.pairs + p0;
-    if (a.interleaved) {
+  }
+  unsigned char* out_q = static_cast<unsigned char*>(a.side[0].out) + int64_t(t) * a.side[0].out_token * kSize;
+  unsigned char* out_k = static_cast<unsigned char*>(a.side[1].out) + int64_t(t) * a.side[1].out_token * kSize;
+  const int64_t oq = a.side[0].out_head * kSize, ok = a.side[1].out_head * kSize;
+  auto stream = [&](auto inter_) {
+    constexpr bool kInter = decltype(inter_)::value;
+    float2 ca[4], sb[4], cb[4], sa[4];
+    int side = -1;
+    // every lane stays for the shuffles
+    for (int hb = 0; hb < heads; hb += kAhead * hp) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < n_rot) {
-          const float2 r = cs[j];
-          const float xr = x[2 * j], xi = x[2 * j + 1];
-          x[2 * j] = fmaf(xr, r.x, -xi * r.y);
-          x[2 * j + 1] = fmaf(xi, r.x, xr * r.y);
+      for (int b = 0; b < kAhead; ++b) {
+        const int h = hb + h0 + b * hp;
+        const bool have = live && h < heads;
+        const int sd = h < q_heads ? 0 : 1;
+        if (sd != side) {  // the coefficients of q's or k's gains
+          side = sd;
+          const void* weight = a.norm ? (sd ? a.side[1].weight : a.side[0].weight) : nullptr;
+          float w[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = 1.0f;
+          if (weight) {
+            unpack<DT>(load_chunk<DT>(weight, 8 * c0), w);
+            unpack<DT>(load_chunk<DT>(weight, 8 * c1), w + 8);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float wa = w[ia(j, kInter)], wb = w[ib(j, kInter)];
+            float* pc = reinterpret_cast<float*>(ca) + j;
+            *pc = wa * cs[j].x;
+            reinterpret_cast<float*>(sb)[j] = -wb * cs[j].y;
+            reinterpret_cast<float*>(cb)[j] = wb * cs[j].x;
+            reinterpret_cast<float*>(sa)[j] = wa * cs[j].y;
+          }
         }
-    } else if (n_rot) {
+        float x[16];
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        if (have) {
+          arrived(b, 0, x);
+          arrived(b, 1, x + 8);
+        } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 r = cs[j];
-        const float xr = x[j], xi = x[8 + j];
-        x[j] = fmaf(xr, r.x, -xi * r.y);
-        x[8 + j] = fmaf(xi, r.x, xr * r.y);
+          for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+        }
+        request(b, h + kAhead * hp);
+        float2 A[4], Bv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          A[j] = make_float2(x[ia(2 * j, kInter)], x[ia(2 * j + 1, kInter)]);
+          Bv[j] = make_float2(x[ib(2 * j, kInter)], x[ib(2 * j + 1, kInter)]);
+        }
+        float inv = 1.0f;
+        if (a.norm) {
+          float2 s0 = __fmul2_rn(A[0], A[0]), s1 = __fmul2_rn(Bv[0], Bv[0]);
+#pragma unroll
+          for (int j = 1; j < 4; ++j) {
+            s0 = __ffma2_rn(A[j], A[j], s0);
+            s1 = __ffma2_rn(Bv[j], Bv[j], s1);
+          }
+          const float2 s = __fadd2_rn(s0, s1);
+          float ss = s.x + s.y;
+#pragma unroll
+          for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, d);
+          inv = rsqrtf(fmaf(ss, 1.0f / D, a.eps));
+        }
+        if (!have) continue;
+        const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 ra = __ffma2_rn(Bv[j], sb[j], __fmul2_rn(A[j], ca[j]));
+          const float2 rb = __ffma2_rn(A[j], sa[j], __fmul2_rn(Bv[j], cb[j]));
+          float2 na = __fmul2_rn(ra, inv2), nb = __fmul2_rn(rb, inv2);
+          if (rotates != 0xFFu) {
+            const float2 ta = __fmul2_rn(__fmul2_rn(A[j], ca[j]), inv2), tb = __fmul2_rn(__fmul2_rn(Bv[j], cb[j]), inv2);
+            if (!(rotates >> (2 * j) & 1u)) na.x = ta.x, nb.x = tb.x;
+            if (!(rotates >> (2 * j + 1) & 1u)) na.y = ta.y, nb.y = tb.y;
+          }
+          x[ia(2 * j, kInter)] = na.x, x[ia(2 * j + 1, kInter)] = na.y;
+          x[ib(2 * j, kInter)] = nb.x, x[ib(2 * j + 1, kInter)] = nb.y;
+        }
+        unsigned char* row = sd == 0 ? out_q + int64_t(h) * oq : out_k + int64_t(h - q_heads) * ok;
+        store_chunk<DT>(row, 8 * c0, x);
+        store_chunk<DT>(row, 8 * c1, x + 8);
       }
     }
-    const int64_t base = int64_t(t0 + uint64_t(t)) * S.out_token + int64_t(h) * S.out_head;
-    store_chunk<DT>(S.out, base + 8 * c0, x);
-    store_chunk<DT>(S.out, base + 8 * c1, x + 8);
-  }
+  };
+  if (a.interleaved) stream(std::true_type());
+  else stream(std::false_type());
 }
 
 // Any even head_dim up to kRotaryMaxDim, any strides: one warp per (token,
@@ -251,7 +355,7 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary_any(const RotaryParams a
   const RopePositions& P = a.pos;
   const uint64_t t0 = uint64_t(blockIdx.x) * uint64_t(a.tokens_per_cta);
   const int nt = int(min(uint64_t(a.tokens_per_cta), a.tokens - t0));
-  fill_angles(P, table, t0, nt);
+  for_angles(P, t0, nt, [&](int t, int p, float2 cs) { table[t * P.pairs + p] = cs; });
   __syncthreads();
   const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
   const int heads = a.side[0].heads + a.side[1].heads, slots = a.D / 2;
@@ -326,8 +430,11 @@ cudaError_t launch_rope_tables(const RopePositions& p, uint64_t tokens, float* c
                                cudaStream_t s) {
   const uint64_t total = tokens * uint64_t(p.pairs);
   if (total == 0) return cudaSuccess;
-  const uint64_t ctas = (total + kRotThreads - 1) / kRotThreads;
-  k_rope_tables<<<unsigned(ctas < 148 * 32 ? ctas : 148 * 32), kRotThreads, 0, s>>>(p, tokens, cos_out, sin_out);
+  // a few angles per thread, and CTAs for every SM
+  const uint64_t rows = uint64_t(kRotThreads / (p.pairs < kRotThreads ? p.pairs : kRotThreads));
+  uint64_t per = (tokens + 148 * 8 - 1) / (148 * 8);
+  per = (per + rows - 1) / rows * rows;
+  k_rope_tables<<<unsigned((tokens + per - 1) / per), kRotThreads, 0, s>>>(p, tokens, int(per), cos_out, sin_out);
   return cudaGetLastError();
 }
 
@@ -344,14 +451,22 @@ cudaError_t launch_rotary(RotaryParams a, int dtype, cudaStream_t s) {
                            uintptr_t((sd.in_token | sd.in_head | sd.out_token | sd.out_head) * int64_t(es));
     if (bits & 15u) vec = false;
   }
-  // Tokens per CTA: enough rows that a CTA's angles (about one per thread)
-  // serve several rows per thread, and at most 32.
-  const int lanes = vec ? a.D / 16 : 32;
-  int nt = (4 * kRotThreads + heads * lanes - 1) / (heads * lanes);
-  nt = nt < 1 ? 1 : nt > 32 ? 32 : nt;
-  a.tokens_per_cta = nt;
-  const uint64_t grid = (a.tokens + uint64_t(nt) - 1) / uint64_t(nt);
-  const size_t smem = size_t(nt) * a.pos.pairs * sizeof(float2);  // <= 32 * 128 * 8 = 32 KB
+  uint64_t grid;
+  size_t smem = 0;
+  if (vec) {
+    // groups per token: enough for some 768 threads an SM, at least three rows each
+    const int lanes = a.D / 16;
+    a.log_hp = 0;
+    while ((a.tokens << a.log_hp) * uint64_t(lanes) < 148 * 768 && (heads >> a.log_hp) > 3) ++a.log_hp;
+    grid = ((a.tokens << a.log_hp) * uint64_t(lanes) + kRotThreads - 1) / kRotThreads;
+  } else {
+    // a row per warp: enough rows that a CTA's angles serve several
+    int nt = (4 * kRotThreads + heads * 32 - 1) / (heads * 32);
+    nt = nt < 1 ? 1 : nt > 32 ? 32 : nt;
+    a.tokens_per_cta = nt;
+    grid = (a.tokens + uint64_t(nt) - 1) / uint64_t(nt);
+    smem = size_t(nt) * a.pos.pairs * sizeof(float2);  // <= 32 * 128 * 8 = 32 KB
+  }
   switch (dtype) {
     case F32: return launch_dt<F32>(a, vec, unsigned(grid), smem, s);
     case BF16: return launch_dt<BF16>(a, vec, unsigned(grid), smem, s);

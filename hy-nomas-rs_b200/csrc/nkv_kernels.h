@@ -292,6 +292,7 @@ struct RotaryParams {
   int32_t norm;
   float eps;
   int32_t tokens_per_cta;  // set by the launcher
+  int32_t log_hp;          // set by the launcher
 };
 cudaError_t launch_rotary(RotaryParams a, int dtype, cudaStream_t s);
 
