@@ -44,25 +44,40 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 bool float_type(int32_t dt) { return dt == NKV_F32 || dt == NKV_BF16 || dt == NKV_F16; }
 
+// The axes' pairs and frequencies.  The last configuration's are kept per
+// thread: 64 powers take longer than a small call's other host work.
 nkv::RopePositions rope_positions(const nkv_rope_axes& ax, const void* positions, int32_t type) {
   if (ax.n_axes < 1 || ax.n_axes > 4) fail(NKV_ERR_INVALID_CONFIG, "rotary positions need 1 to 4 axes");
   if (!(ax.theta > 0.0) || !std::isfinite(ax.theta))
     fail(NKV_ERR_INVALID_CONFIG, "theta must be finite and positive");
   if (type < NKV_POS_I32 || type > NKV_POS_F32)
     fail(NKV_ERR_ARGUMENT, "unknown position type " + std::to_string(type));
-  nkv::RopePositions p{};
+  struct Known {
+    int32_t n_axes = 0, dims[4] = {0, 0, 0, 0};
+    double theta = 0.0;
+    nkv::RopePositions p{};
+  };
+  static thread_local Known known;
+  if (known.n_axes != ax.n_axes || known.theta != ax.theta || !std::equal(ax.dims, ax.dims + ax.n_axes, known.dims)) {
+    nkv::RopePositions p{};
+    p.n_axes = ax.n_axes;
+    for (int a = 0; a < ax.n_axes; ++a) {
+      const int32_t d = ax.dims[a];
+      if (d < 2 || d % 2 || d > nkv::kRotaryMaxDim || p.pairs + d / 2 > nkv::kRotaryMaxDim / 2)
+        fail(NKV_ERR_INVALID_CONFIG, "rotary axes need even dims >= 2 with a sum of at most 256");
+      for (int i = 0; i < d / 2; ++i) {
+        p.axis[p.pairs] = uint8_t(a);
+        p.freq[p.pairs++] = std::pow(ax.theta, -2.0 * i / d);
+      }
+    }
+    known.n_axes = ax.n_axes;
+    std::copy(ax.dims, ax.dims + ax.n_axes, known.dims);
+    known.theta = ax.theta;
+    known.p = p;
+  }
+  nkv::RopePositions p = known.p;
   p.data = positions;
   p.dtype = type;
-  p.n_axes = ax.n_axes;
-  for (int a = 0; a < ax.n_axes; ++a) {
-    const int32_t d = ax.dims[a];
-    if (d < 2 || d % 2 || d > nkv::kRotaryMaxDim || p.pairs + d / 2 > nkv::kRotaryMaxDim / 2)
-      fail(NKV_ERR_INVALID_CONFIG, "rotary axes need even dims >= 2 with a sum of at most 256");
-    for (int i = 0; i < d / 2; ++i) {
-      p.axis[p.pairs] = uint8_t(a);
-      p.freq[p.pairs++] = std::pow(ax.theta, -2.0 * i / d);
-    }
-  }
   return p;
 }
 

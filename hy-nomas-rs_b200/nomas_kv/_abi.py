@@ -224,9 +224,10 @@ SIGNATURES = {
     "nkv_qvg_decode": (C.c_int, [P, I32, P, P, U64, I64, I64, I32, I32, I32, P, P]),
     "nkv_synth_fill": (C.c_int, [P, I32, U64, I64, I64, U64, U64, P, P, P]),
     "nkv_kv_project": (C.c_int, [C.POINTER(nkv_kv_project_args), P]),
-    "nkv_rope_tables": (C.c_int, [C.POINTER(nkv_rope_axes), P, I32, U64, P, P, P]),
-    "nkv_rotary": (C.c_int, [C.POINTER(nkv_rotary_args), P]),
-    "nkv_residual_norm": (C.c_int, [C.POINTER(nkv_residual_norm_args), P]),
+    # the block operators' argument structs are passed packed (block.py) or by reference
+    "nkv_rope_tables": (C.c_int, [P, P, I32, U64, P, P, P]),
+    "nkv_rotary": (C.c_int, [P, P]),
+    "nkv_residual_norm": (C.c_int, [P, P]),
     "nkv_attend_plan_create": (C.c_int, [C.POINTER(U64), C.POINTER(U64), U64, I32, I32, I32, I32, U64, I32,
                                          C.POINTER(P)]),
     "nkv_attend_plan_destroy": (C.c_int, [P]),
@@ -234,7 +235,7 @@ SIGNATURES = {
     "nkv_attend_plan_status": (C.c_int, [P, C.POINTER(C.c_uint32)]),
     "nkv_attend_schedule": (C.c_int, [C.POINTER(U64), C.POINTER(U64), U64, I32, I32, I32, U64, I32, P, U64,
                                       C.POINTER(U64)]),
-    "nkv_attend_packed": (C.c_int, [P, C.POINTER(nkv_attend_args), P]),
+    "nkv_attend_packed": (C.c_int, [P, P, P]),
     "nkv_int8_quantize_layers_noalloc": (C.c_int, [C.POINTER(P), C.POINTER(P), I32, I32, U64, I64, C.POINTER(P),
                                                    C.POINTER(P), C.POINTER(P), C.POINTER(P),
                                                    C.POINTER(C.c_uint32), P]),

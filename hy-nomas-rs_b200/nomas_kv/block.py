@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -28,21 +29,42 @@ _NORMS = {None: _abi.NKV_NORM_NONE, "none": _abi.NKV_NORM_NONE, "rms": _abi.NKV_
           "layer": _abi.NKV_NORM_LAYER}
 
 
+# A call of a few microseconds of GPU work is bound by what happens here, so
+# the argument structs are packed in one go (native layout, as the header's)
+# and the checks read each attribute once.
+_AXES = struct.Struct("i4iid")
+_ROTARY = struct.Struct("32sPiiQiif" + "PPqqqqPi0P" * 2)
+_NORM = struct.Struct("QqiiiiifPPPPqqqqPPPPPPi0P")
+_ATTEND = struct.Struct("iiQQPPPqqqqqqfPPPPPQ")
+for _s, _t in ((_AXES, _abi.nkv_rope_axes), (_ROTARY, _abi.nkv_rotary_args), (_NORM, _abi.nkv_residual_norm_args),
+               (_ATTEND, _abi.nkv_attend_args)):
+    assert _s.size == C.sizeof(_t), _t.__name__
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 # ---------------------------------------------------------------- checks
-def _device_of(first, *rest):
-    """The CUDA device all given tensors are on (None entries skipped)."""
-    dev = first.device
-    if dev.type != "cuda":
+def _device_of(first, *rest) -> int:
+    """The index of the CUDA device all given tensors are on (None entries
+    skipped)."""
+    index = first.get_device()
+    if index < 0:
         raise ArgumentError("the tensors must be on a CUDA device (no CPU fallback)")
     grad = torch.is_grad_enabled()
-    for t in (first, *rest):
+    if grad and first.requires_grad:
+        raise ArgumentError(_NO_GRAD)
+    for t in rest:
         if t is None:
             continue
-        if t.device != dev:
-            raise ArgumentError(f"all tensors must be on {dev}, got one on {t.device}")
+        if t.get_device() != index:
+            raise ArgumentError(f"all tensors must be on {first.device}, got one on {t.device}")
         if grad and t.requires_grad:
-            raise ArgumentError("inference only: an input requires a gradient (use torch.no_grad() or detach())")
-    return dev
+            raise ArgumentError(_NO_GRAD)
+    return index
+
+
+_NO_GRAD = "inference only: an input requires a gradient (use torch.no_grad() or detach())"
 
 
 def _code(t, name: str) -> int:
@@ -52,36 +74,33 @@ def _code(t, name: str) -> int:
     return code
 
 
-class _On:
-    """Device and stream of one call: makes the device current, gives the raw
-    stream, and ties the tensors' memory to it when it is not the current one
-    (the allocator then keeps a tensor freed early until the call's work is
-    done)."""
+class _Elsewhere:
+    """Makes a device current, and a stream other than its current one, whose
+    work the tensors' memory is then tied to (the allocator keeps a tensor
+    freed early until that work is done)."""
 
-    def __init__(self, dev, stream, tensors):
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-        self.dev, self.stream, self.tensors = dev, stream, tensors
+    def __init__(self, index, stream, tensors):
+        self.device = torch.cuda.device(index)
+        self.device.__enter__()
+        self.stream = None
+        if stream is not None and stream != torch.cuda.current_stream(index):
+            self.stream = torch.cuda.stream(stream)
+            self.stream.__enter__()
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(stream)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        current = torch.cuda.current_stream(self.dev)
-        self.switch = None
-        if self.stream is None or self.stream == current:
-            return C.c_void_p(current.cuda_stream)
-        self.switch = torch.cuda.stream(self.stream)
-        self.switch.__enter__()
-        for t in self.tensors:
-            if t is not None:
-                t.record_stream(self.stream)
-        return C.c_void_p(self.stream.cuda_stream)
+    def leave(self):
+        if self.stream is not None:
+            self.stream.__exit__(None, None, None)
+        self.device.__exit__(None, None, None)
 
-    def __exit__(self, *exc):
-        if self.switch is not None:
-            self.switch.__exit__(*exc)
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+
+def _enter(index, stream, tensors):
+    """None where the call runs on the current device's current stream."""
+    if stream is None and torch.cuda.current_device() == index:
+        return None
+    return _Elsewhere(index, stream, tensors)
 
 
 def _extent(t) -> int:
@@ -165,14 +184,15 @@ class RotaryAxes:
         if not (self.theta > 0 and math.isfinite(self.theta)):
             raise InvalidConfigError("theta must be finite and positive")
         object.__setattr__(self, "dims", dims)
+        object.__setattr__(self, "_packed", _AXES.pack(len(dims), *(dims + (0,) * (4 - len(dims))),
+                                                       int(bool(self.interleaved)), float(self.theta)))
 
     @property
     def pairs(self) -> int:
         return sum(self.dims) // 2
 
     def to_c(self) -> _abi.nkv_rope_axes:
-        return _abi.nkv_rope_axes(len(self.dims), (C.c_int32 * 4)(*self.dims), int(self.interleaved),
-                                  float(self.theta))
+        return _abi.nkv_rope_axes.from_buffer_copy(self._packed)
 
 
 def _positions(positions, axes: RotaryAxes, tokens: Optional[int]) -> int:
@@ -191,30 +211,26 @@ def rope_tables(positions, axes: RotaryAxes, cos=None, sin=None, stream=None):
     """The (cos, sin) f32 tables (tokens, axes.pairs) of nkv_rope_tables: what
     kv_project takes as `rope` (64 pairs).  positions: (tokens, n_axes) int32,
     int64 or f32."""
-    dev = _device_of(positions, cos, sin)
+    index = _device_of(positions, cos, sin)
     code = _positions(positions, axes, None)
     shape = (positions.shape[0], axes.pairs)
-    with _On(dev, stream, (positions, cos, sin)) as s:
+    away = _enter(index, stream, (positions, cos, sin))
+    try:
         for name, t, other in (("cos", cos, sin), ("sin", sin, cos)):
             if t is not None:
-                _check_out(t, _Like(shape, torch.float32, dev), (positions,), name, others=(other,))
+                _check_out(t, _Like(shape, torch.float32, positions.device), (positions,), name, others=(other,))
                 if not t.is_contiguous():
                     raise GeometryError(f"{name} must be contiguous")
         if cos is None:
-            cos = torch.empty(shape, dtype=torch.float32, device=dev)
+            cos = positions.new_empty(shape, dtype=torch.float32)
         if sin is None:
-            sin = torch.empty(shape, dtype=torch.float32, device=dev)
-        c = axes.to_c()
-        _check(lib().nkv_rope_tables(C.byref(c), positions.data_ptr(), code, shape[0], cos.data_ptr(),
-                                     sin.data_ptr(), s))
+            sin = positions.new_empty(shape, dtype=torch.float32)
+        _check(lib().nkv_rope_tables(axes._packed, positions.data_ptr(), code, shape[0], cos.data_ptr(),
+                                     sin.data_ptr(), _raw_stream(index)))
+    finally:
+        if away is not None:
+            away.leave()
     return cos, sin
-
-
-def _rotary_side(t, out, weight) -> _abi.nkv_rotary_side:
-    it, ih, _ = t.stride()
-    ot, oh, _ = out.stride()
-    return _abi.nkv_rotary_side(t.data_ptr(), out.data_ptr(), it, ih, ot, oh,
-                                None if weight is None else weight.data_ptr(), t.shape[1])
 
 
 def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=None, k_weight=None,
@@ -226,46 +242,58 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
     dimension dense, so q and k may be views of one fused projection.  q_out /
     k_out may be q / k themselves (in place).  Returns q_out, or (q_out,
     k_out) when k is given."""
-    dev = _device_of(q, k, positions, q_weight, k_weight, q_out, k_out)
+    index = _device_of(q, k, positions, q_weight, k_weight, q_out, k_out)
     code = _code(q, "q")
     if q.dim() != 3:
         raise GeometryError("q must be (tokens, heads, head_dim)")
-    tokens, _, D = q.shape
+    tokens, heads, D = q.shape
     if D < 2 or D % 2 or D > 256:
         raise GeometryError("head_dim must be even, 2 to 256")
     if 2 * axes.pairs > D:
         raise GeometryError(f"rotary axes {axes.dims} exceed head_dim {D}")
-    if k is not None and (k.dim() != 3 or k.shape[0] != tokens or k.shape[2] != D or k.dtype != q.dtype):
+    if k is None:
+        if k_weight is not None or k_out is not None:
+            raise ArgumentError("k_weight and k_out need k")
+    elif k.dim() != 3 or k.shape[0] != tokens or k.shape[2] != D or k.dtype != q.dtype:
         raise GeometryError(f"k must be ({tokens}, kv_heads, {D}) {q.dtype}")
-    if k is None and (k_weight is not None or k_out is not None):
-        raise ArgumentError("k_weight and k_out need k")
     if not norm and (q_weight is not None or k_weight is not None):
         raise ArgumentError("q_weight and k_weight need norm=True")
     pcode = _positions(positions, axes, tokens)
-    for name, t in (("q", q), ("k", k)):
-        if t is not None and t.stride(2) != 1:
-            raise GeometryError(f"the last dimension of {name} must be dense")
+    q_st = q.stride()
+    k_st = (0, 0, 1) if k is None else k.stride()
+    if q_st[2] != 1 or k_st[2] != 1:
+        raise GeometryError("the last dimension of q and k must be dense")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (tuple(w.shape) != (D,) or w.dtype != q.dtype or not w.is_contiguous()):
+        if w is not None and (w.shape != (D,) or w.dtype != q.dtype or not w.is_contiguous()):
             raise GeometryError(f"{name} must be a contiguous ({D},) {q.dtype} tensor")
-    with _On(dev, stream, (q, k, positions, q_weight, k_weight, q_out, k_out)) as s:
+    ins = (q, k, positions, q_weight, k_weight)
+    away = _enter(index, stream, (*ins, q_out, k_out))
+    try:
         if q_out is not None:
-            _check_out(q_out, q, (q, k, positions, q_weight, k_weight), "q_out", alias=(q,), others=(k_out,))
+            _check_out(q_out, q, ins, "q_out", alias=(q,), others=(k_out,))
+            qo_st = q_out.stride()
         else:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            q_out = q.new_empty(q.shape)
+            qo_st = (heads * D, D)
+        k_heads, k_p, ko_p, ko_st = 0, 0, 0, (0, 0)
         if k is not None:
+            k_heads = k.shape[1]
             if k_out is not None:
-                _check_out(k_out, k, (k, q, positions, q_weight, k_weight), "k_out", alias=(k,), others=(q_out,))
+                _check_out(k_out, k, ins, "k_out", alias=(k,), others=(q_out,))
+                ko_st = k_out.stride()
             else:
-                k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        a = _abi.nkv_rotary_args()
-        a.axes = axes.to_c()
-        a.positions, a.position_type, a.dtype = positions.data_ptr(), pcode, code
-        a.tokens, a.head_dim, a.norm, a.eps = tokens, D, int(bool(norm)), float(eps)
-        a.q = _rotary_side(q, q_out, q_weight)
-        if k is not None:
-            a.k = _rotary_side(k, k_out, k_weight)
-        _check(lib().nkv_rotary(C.byref(a), s))
+                k_out = k.new_empty(k.shape)
+                ko_st = (k_heads * D, D)
+            k_p, ko_p = k.data_ptr(), k_out.data_ptr()
+        _check(lib().nkv_rotary(
+            _ROTARY.pack(axes._packed, positions.data_ptr(), pcode, code, tokens, D, 1 if norm else 0, eps,
+                         q.data_ptr(), q_out.data_ptr(), q_st[0], q_st[1], qo_st[0], qo_st[1],
+                         0 if q_weight is None else q_weight.data_ptr(), heads,
+                         k_p, ko_p, k_st[0], k_st[1], ko_st[0], ko_st[1],
+                         0 if k_weight is None else k_weight.data_ptr(), k_heads), _raw_stream(index)))
+    finally:
+        if away is not None:
+            away.leave()
     return q_out if k is None else (q_out, k_out)
 
 
@@ -274,7 +302,7 @@ def _vector(t, name: str, dim: int, dtype, seen):
     """A weight of `dim` values, f32 or the stream's dtype, like the others."""
     if t is None:
         return seen
-    if tuple(t.shape) != (dim,) or not t.is_contiguous():
+    if t.shape != (dim,) or not t.is_contiguous():
         raise GeometryError(f"{name} must be a contiguous ({dim},) tensor")
     if t.dtype not in (torch.float32, dtype) or (seen is not None and t.dtype != seen):
         raise GeometryError(f"the weights must share one type, f32 or {dtype}")
@@ -295,7 +323,7 @@ def residual_norm(x, branch=None, *, gate=None, post=None, post_weight=None, nor
     index is out of range gets NaN).  Without a branch h is x; with norm None
     y is None.  h_out / y_out may be x or branch.  Returns (h, y); y is what
     kv_project takes as x."""
-    dev = _device_of(x, branch, gate, post_weight, weight, scale, shift, mod_index, h_out, y_out)
+    index = _device_of(x, branch, gate, post_weight, weight, scale, shift, mod_index, h_out, y_out)
     code = _code(x, "x")
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise GeometryError("x must be (tokens, dim) with dense rows")
@@ -329,38 +357,39 @@ def residual_norm(x, branch=None, *, gate=None, post=None, post_weight=None, nor
             raise GeometryError("gate, scale and shift must have the same number of rows")
         mdt, groups = t.dtype, g
     if mod_index is not None:
-        if tuple(mod_index.shape) != (tokens,) or mod_index.dtype != torch.int32 or not mod_index.is_contiguous():
+        if mod_index.shape != (tokens,) or mod_index.dtype != torch.int32 or not mod_index.is_contiguous():
             raise GeometryError(f"mod_index must be a contiguous ({tokens},) int32 tensor")
         if not groups:
             raise ArgumentError("mod_index needs gate, scale or shift")
     elif groups > 1:
         raise GeometryError("several modulation rows need mod_index")
     vectors = (gate, post_weight, weight, scale, shift, mod_index)
-    with _On(dev, stream, (x, branch, h_out, y_out, *vectors)) as s:
-        h, y = x, None
+    away = _enter(index, stream, (x, branch, h_out, y_out, *vectors))
+    try:
+        h, y, h_p, y_p, h_st, y_st = x, None, 0, 0, 0, 0
         if branch is not None:
             if h_out is not None:
                 _check_out(h_out, x, (x, branch, *vectors), "h_out", alias=(x, branch), others=(y_out,))
-            h = torch.empty((tokens, dim), dtype=x.dtype, device=dev) if h_out is None else h_out
+                h, h_st = h_out, h_out.stride(0)
+            else:
+                h, h_st = x.new_empty((tokens, dim)), dim
+            h_p = h.data_ptr()
         if norm_c:
             if y_out is not None:
                 _check_out(y_out, x, (x, branch, *vectors), "y_out", alias=(x, branch), others=(h_out,))
-            y = torch.empty((tokens, dim), dtype=x.dtype, device=dev) if y_out is None else y_out
-        p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        a = _abi.nkv_residual_norm_args()
-        a.tokens, a.dim, a.dtype = tokens, dim, code
-        a.weight_dtype = code if wdt is None else _CODES[wdt]
-        a.mod_dtype = code if mdt is None else _CODES[mdt]
-        a.post, a.norm, a.eps = post_c, norm_c, float(eps)
-        a.x, a.x_stride = x.data_ptr(), x.stride(0)
-        if branch is not None:
-            a.branch, a.branch_stride = branch.data_ptr(), branch.stride(0)
-            a.h_out, a.h_stride = h.data_ptr(), h.stride(0)
-        if norm_c:
-            a.y_out, a.y_stride = y.data_ptr(), y.stride(0)
-        a.post_weight, a.weight, a.gate, a.scale, a.shift = p(post_weight), p(weight), p(gate), p(scale), p(shift)
-        a.mod_index, a.mod_rows = p(mod_index), groups
-        _check(lib().nkv_residual_norm(C.byref(a), s))
+                y, y_st = y_out, y_out.stride(0)
+            else:
+                y, y_st = x.new_empty((tokens, dim)), dim
+            y_p = y.data_ptr()
+        p = [0 if t is None else t.data_ptr() for t in vectors]
+        _check(lib().nkv_residual_norm(
+            _NORM.pack(tokens, dim, code, code if wdt is None else _CODES[wdt], code if mdt is None else _CODES[mdt],
+                       post_c, norm_c, eps, x.data_ptr(), 0 if branch is None else branch.data_ptr(), h_p, y_p,
+                       x.stride(0), 0 if branch is None else branch.stride(0), h_st, y_st, p[1], p[2], p[0], p[3],
+                       p[4], p[5], groups), _raw_stream(index)))
+    finally:
+        if away is not None:
+            away.leave()
     return h, y
 
 
@@ -448,59 +477,63 @@ def attend_packed(plan: AttendPlan, q, k, v, scale: Optional[float] = None, hist
         raise ArgumentError("the plan is closed")
     H, KV, D = plan.heads, plan.kv_heads, plan.head_dim
     ho, hl = (None, None) if history is None else history
-    dev = _device_of(q, k, v, ho, hl, out, lse)
-    if dev != plan.device:
-        raise ArgumentError(f"the plan is for {plan.device}, the tensors are on {dev}")
+    index = _device_of(q, k, v, ho, hl, out, lse)
+    if index != plan.device.index:
+        raise ArgumentError(f"the plan is for {plan.device}, the tensors are on {q.device}")
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise GeometryError("packed attention needs bf16 or f16 queries, keys and values")
     if q.dim() != 3 or q.shape[1:] != (H, D) or q.shape[0] < plan.q_tokens:
         raise GeometryError(f"q must be (at least {plan.q_tokens}, {H}, {D})")
-    rows, k_rows = q.shape[0], k.shape[0] if k.dim() else 0
+    rows = q.shape[0]
     for name, t in (("k", k), ("v", v)):
         if t.dim() != 3 or t.shape[1:] != (KV, D) or t.shape[0] < plan.k_tokens or t.dtype != q.dtype:
             raise GeometryError(f"{name} must be (at least {plan.k_tokens}, {KV}, {D}) {q.dtype}")
-    k_rows = min(k_rows, v.shape[0])
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.stride(2) != 1:
+    k_rows = min(k.shape[0], v.shape[0])
+    where = []  # address, token stride, head stride
+    for name, t, heads in (("q", q, H), ("k", k, KV), ("v", v, KV)):
+        p, (st, sh, sd) = t.data_ptr(), t.stride()
+        if sd != 1:
             raise GeometryError(f"the last dimension of {name} must be dense")
         # a dimension of one has no stride that counts
-        if t.numel() and (t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 8) or
-                          (t.shape[1] > 1 and t.stride(1) % 8)):
+        if t.shape[0] < 2:
+            st = 0
+        if heads < 2:
+            sh = 0
+        if (p | st * 2 | sh * 2) % 16:
             raise ArgumentError(f"{name} must be 16-byte aligned with strides of multiples of 8 elements")
+        where.append((p, st, sh))
+    ho_p = hl_p = 0
     if history is not None:
         for name, t, shape in (("o", ho, (rows, H, D)), ("lse", hl, (H, rows))):
-            if tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous():
+            if t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous():
                 raise GeometryError(f"the history's {name} must be a contiguous f32 tensor of shape {shape}")
-    with _On(dev, stream, (q, k, v, ho, hl, out, lse)) as s:
+        ho_p, hl_p = ho.data_ptr(), hl.data_ptr()
+    away = _enter(index, stream, (q, k, v, ho, hl, out, lse))
+    try:
+        padded = rows != plan.q_tokens
         if out is None:
             # a padded batch keeps rows that nothing writes: zeros, not stale memory
-            new = torch.empty if rows == plan.q_tokens else torch.zeros
-            out = new((rows, H, D), dtype=q.dtype, device=dev)
+            out = q.new_zeros((rows, H, D)) if padded else q.new_empty((rows, H, D))
         else:
-            like = _Like((rows, H, D), torch.float32 if out.dtype == torch.float32 else q.dtype, dev)
+            like = _Like((rows, H, D), torch.float32 if out.dtype == torch.float32 else q.dtype, q.device)
             _check_out(out, like, (q, k, v, ho, hl), "out", others=(lse,))
             if not out.is_contiguous():
                 raise GeometryError("out must be contiguous")
         if lse is None:
-            lse = torch.empty((H, rows), dtype=torch.float32, device=dev) if rows == plan.q_tokens else \
-                torch.full((H, rows), -math.inf, dtype=torch.float32, device=dev)
+            lse = q.new_full((H, rows), -math.inf, dtype=torch.float32) if padded else \
+                q.new_empty((H, rows), dtype=torch.float32)
         else:
-            _check_out(lse, _Like((H, rows), torch.float32, dev), (q, k, v, ho, hl), "lse", others=(out,))
+            _check_out(lse, _Like((H, rows), torch.float32, q.device), (q, k, v, ho, hl), "lse", others=(out,))
             if not lse.is_contiguous():
                 raise GeometryError("lse must be contiguous")
-        ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=dev) if plan.workspace_bytes else None
-        a = _abi.nkv_attend_args()
-        a.dtype, a.out_dtype = _CODES[q.dtype], _CODES[out.dtype]
-        a.q_rows, a.k_rows = rows, k_rows
-        one = lambda t, i: t.stride(i) if t.shape[i] > 1 else 0  # noqa: E731
-        a.q, a.q_token_stride, a.q_head_stride = q.data_ptr(), one(q, 0), one(q, 1)
-        a.k, a.k_token_stride, a.k_head_stride = k.data_ptr(), one(k, 0), one(k, 1)
-        a.v, a.v_token_stride, a.v_head_stride = v.data_ptr(), one(v, 0), one(v, 1)
-        a.scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-        a.out, a.lse = out.data_ptr(), lse.data_ptr()
-        if ho is not None:
-            a.hist_out, a.hist_lse = ho.data_ptr(), hl.data_ptr()
-        if ws is not None:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), plan.workspace_bytes
-        _check(lib().nkv_attend_packed(plan._h, C.byref(a), s))
+        n = plan.workspace_bytes
+        ws = q.new_empty(n, dtype=torch.uint8) if n else None
+        (qp, qt, qh), (kp, kt, kh), (vp, vt, vh) = where
+        _check(lib().nkv_attend_packed(
+            plan._h, _ATTEND.pack(_CODES[q.dtype], _CODES[out.dtype], rows, k_rows, qp, kp, vp, qt, qh, kt, kh, vt, vh,
+                                  1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(), lse.data_ptr(),
+                                  ho_p, hl_p, ws.data_ptr() if n else 0, n), _raw_stream(index)))
+    finally:
+        if away is not None:
+            away.leave()
     return out, lse
