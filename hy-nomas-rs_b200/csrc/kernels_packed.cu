@@ -475,12 +475,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t bits = 0;
     for (int i = first; i < last && ok; ++i) {
       int nh, lim;  // the half's steps; the row's visible keys, from the item's first tile
+      bool idle;    // no row of the warp's: it only hands its part of P over
       {
         const PackedItem it = read_item(a.items + i);
         nh = hf ? it.steps1 : it.steps0;
         const int jt = int((uint32_t(row) * a.g_magic) >> 16);  // row / G
-        const bool have = row < min(a.half_rows, it.rows - hf * a.half_rows);
-        lim = have ? key_limit(a, it, (it.row0 + hf * a.half_rows) / G + jt) - it.t_lo * PK : 0;
+        const int n_rows = min(a.half_rows, it.rows - hf * a.half_rows);
+        // lanes without a row mask nothing: their scores and output are never
+        // kept, and a few of them must not send the warp through the masks
+        lim = row < n_rows ? key_limit(a, it, (it.row0 + hf * a.half_rows) / G + jt) - it.t_lo * PK : 1 << 30;
+        idle = (warp & 3) * 32 >= n_rows;
         const uint32_t tiles = uint32_t((max(it.steps0, it.steps1) + 1) / 2);
         bits = (bits & 31u) | ((((bits >> 5) + tiles) & 3u) << 5);
       }
@@ -504,8 +508,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         return r;
       };
       bool before_seen = false;  // the last PV but one of this item
-      if (nh > 0 && scores_full(0, false)) request(0);
-      for (int u = 0; u < nh && ok; ++u) {
+      for (int u = 0; idle && u < nh && scores_full(u, false); ++u) arrive_lane0(B(kP + 2 * hf + (u & 1)), lane);
+      if (!idle && nh > 0 && scores_full(0, false)) request(0);
+      for (int u = 0; !idle && u < nh && ok; ++u) {
         const int buf = u & 1;
         tmem_load_wait();
         tmem_regs_after_wait(sv);

@@ -32,11 +32,11 @@ inline int64_t packed_key_limit(int64_t q_len, int64_t k_len, bool causal, int64
 
 namespace packed_detail {
 
-// Relative costs, in key tiles of an item with two halves: a tile of an item
-// with one half takes about 0.7 (two halves hide each other's latencies), an
-// item 1.5 for what its start and end do not hide, a partial block of rows 1
-// more to write and merge, the merge's launch 3.
-constexpr double kHalfTile = 0.7, kItem = 1.5, kPart = 1.0, kMerge = 3.0;
+// Relative costs, in key tiles of an item with two halves (about 1.5 us): a
+// tile of an item with one half takes 0.85 (two halves hide each other's
+// latencies), an item 1.5 for what its start and end do not hide, a block of
+// partial rows 1 more to write and merge, the merge's launch 3.
+constexpr double kHalfTile = 0.85, kItem = 1.5, kPart = 1.0, kMerge = 3.0;
 
 struct Unit {
   PackedItem it;  // t_hi = tiles of the unit

@@ -96,6 +96,12 @@ class _Elsewhere:
         self.device.__exit__(None, None, None)
 
 
+def _fresh(like):
+    """A contiguous tensor of like's shape and type (empty_like is the quicker
+    call, but keeps the strides of a dense one)."""
+    return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
+
+
 def _enter(index, stream, tensors):
     """None where the call runs on the current device's current stream."""
     if stream is None and torch.cuda.current_device() == index:
@@ -273,7 +279,7 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
             _check_out(q_out, q, ins, "q_out", alias=(q,), others=(k_out,))
             qo_st = q_out.stride()
         else:
-            q_out = q.new_empty(q.shape)
+            q_out = _fresh(q)
             qo_st = (heads * D, D)
         k_heads, k_p, ko_p, ko_st = 0, 0, 0, (0, 0)
         if k is not None:
@@ -282,7 +288,7 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
                 _check_out(k_out, k, ins, "k_out", alias=(k,), others=(q_out,))
                 ko_st = k_out.stride()
             else:
-                k_out = k.new_empty(k.shape)
+                k_out = _fresh(k)
                 ko_st = (k_heads * D, D)
             k_p, ko_p = k.data_ptr(), k_out.data_ptr()
         _check(lib().nkv_rotary(
@@ -372,14 +378,14 @@ def residual_norm(x, branch=None, *, gate=None, post=None, post_weight=None, nor
                 _check_out(h_out, x, (x, branch, *vectors), "h_out", alias=(x, branch), others=(y_out,))
                 h, h_st = h_out, h_out.stride(0)
             else:
-                h, h_st = x.new_empty((tokens, dim)), dim
+                h, h_st = _fresh(x), dim
             h_p = h.data_ptr()
         if norm_c:
             if y_out is not None:
                 _check_out(y_out, x, (x, branch, *vectors), "y_out", alias=(x, branch), others=(h_out,))
                 y, y_st = y_out, y_out.stride(0)
             else:
-                y, y_st = x.new_empty((tokens, dim)), dim
+                y, y_st = _fresh(x), dim
             y_p = y.data_ptr()
         p = [0 if t is None else t.data_ptr() for t in vectors]
         _check(lib().nkv_residual_norm(
@@ -513,7 +519,7 @@ def attend_packed(plan: AttendPlan, q, k, v, scale: Optional[float] = None, hist
         padded = rows != plan.q_tokens
         if out is None:
             # a padded batch keeps rows that nothing writes: zeros, not stale memory
-            out = q.new_zeros((rows, H, D)) if padded else q.new_empty((rows, H, D))
+            out = q.new_zeros((rows, H, D)) if padded else _fresh(q)
         else:
             like = _Like((rows, H, D), torch.float32 if out.dtype == torch.float32 else q.dtype, q.device)
             _check_out(out, like, (q, k, v, ho, hl), "out", others=(lse,))
