@@ -93,6 +93,20 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// Bounded wait as tc::bar_wait, but small: the roles' code runs from the
+// instruction cache at once, and two dozen waits with their retries unrolled
+// made it 120 KB.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+  if (bar_try(bar, parity)) return true;
+  const uint64_t t0 = gtimer();
+  uint32_t tries = 0;
+#pragma unroll 1
+  do {
+    if (bar_try(bar, parity)) return true;
+  } while ((++tries & 31u) || gtimer() - t0 <= kWaitNs);
+  return false;
+}
+
 // Lane 0's arrival, predicated rather than branched around.
 __device__ __forceinline__ void arrive_lane0(uint32_t bar, int lane) {
   asm volatile(
@@ -220,6 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (tid == 32 * kTmaWarp) {
     // arrivals per phase: P, O free and history read by the half's 4 warps, K / V empty by both MMA warps, else 1
+#pragma unroll 1
     for (int i = 0; i < kBarCount; ++i) {
       const bool by_half = (i >= kP && i < kP + 4) || (i >= kOf && i < kOf + 2) || (i >= kHr && i < kHr + 4);
       const int count = by_half ? 4 : (i >= kKe && i < kKe + NST) || i >= kVe ? 2 : 1;
@@ -251,13 +266,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto wait = [&](int i, uint32_t parity) {
       bool r = __all_sync(0xFFFFFFFFu, bar_try(B(i), parity));
       if (!r) {
-        r = __all_sync(0xFFFFFFFFu, bar_wait(B(i), parity));
+        r = __all_sync(0xFFFFFFFFu, wait_for(B(i), parity));
         if (!r) fail();
       }
       tc_after();
       return r;
     };
     uint32_t tiles = 0, use0 = 0, use1 = 0;  // K / V tiles and uses of the score buffers so far
+#pragma unroll 1
     for (int i = first; i < last && ok; ++i) {
       const PackedItem& it = a.items[i];
       const int n0 = it.steps0, n1 = it.steps1, nh = hf ? n1 : n0, n = (max(n0, n1) + 1) / 2;
@@ -295,6 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (i > first && !wait(kOf + hf, item_ph ^ 1u)) break;
       // One round per tile; this half may need fewer steps than the other, but
       // returns every stage to the rings.
+#pragma unroll 1
       for (int t = 0; t < n && ok; ++t) {
         const int u = 2 * t;
         const uint32_t x = tiles + uint32_t(t), st = x % NST, next = (x + 1) % NST;
@@ -327,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t held = 0, parity = 0;  // per V stage (4 bits): free 0, a tile 1, history columns 2 + e; loads of e modulo 2
       const uint32_t q_bytes = uint32_t(DP / 64) * uint32_t(a.half_rows) * 128u;
       auto wait = [&](int i, uint32_t parity) {
-        if (ok && !bar_wait(B(i), parity)) fail();
+        if (ok && !wait_for(B(i), parity)) fail();
         return ok && *abort_flag == 0u;
       };
       auto load_k = [&](const PackedItem& it, int t) {
@@ -367,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // behind the sequence belong to rows that are not kept
       auto load_q = [&](int i) {
         const PackedItem& it = a.items[i];
+#pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
           if (i > first && !wait(kQe + hf, uint32_t(i - first - 1) & 1u)) return false;
           bar_expect_tx(B(kQf + hf), q_bytes);
@@ -378,6 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       auto load_history = [&](const PackedItem& it) {
+#pragma unroll 1
         for (int e = 0; e < 4; ++e) {  // half e / 2, columns (e & 1) * DP / 2
           const uint32_t st = slots % NST;
           if (!slot_free(st, 2u + uint32_t(e))) return false;
@@ -399,10 +418,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         load_q(first);
       }
       int qs = first < last ? 1 : 0;
-      for (int i = first; i < last && ok; ++i) {
+  #pragma unroll 1
+    for (int i = first; i < last && ok; ++i) {
         const PackedItem it = a.items[i];
         const int n = tiles_of(it);
         bool run = true;
+#pragma unroll 1
         for (int t = 0; t < n && run; ++t) run = load_v(it, t) && (t + 1 == n || load_k(it, t + 1));
         if (run && i + 1 < last) {
           run = (tiles_of(a.items[i + 1]) == 0 || load_k(a.items[i + 1], 0)) && load_q(i + 1);
@@ -413,23 +434,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // no copy in flight when the CTA ends: wait (bounded) for the last load
       // on every barrier; on the normal path they have all been consumed
-      for (uint32_t x = kt > NST ? kt - NST : 0; x < kt; ++x) bar_wait(B(kKf + x % NST), (x / NST) & 1u);
-      for (uint32_t x = vt > NST ? vt - NST : 0; x < vt; ++x) bar_wait(B(kVf + x % NST), (x / NST) & 1u);
+#pragma unroll 1
+      for (uint32_t x = kt > NST ? kt - NST : 0; x < kt; ++x) wait_for(B(kKf + x % NST), (x / NST) & 1u);
+#pragma unroll 1
+      for (uint32_t x = vt > NST ? vt - NST : 0; x < vt; ++x) wait_for(B(kVf + x % NST), (x / NST) & 1u);
       if (qs)
-        for (int hf = 0; hf < 2; ++hf) bar_wait(B(kQf + hf), uint32_t(qs - 1) & 1u);
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) wait_for(B(kQf + hf), uint32_t(qs - 1) & 1u);
       if (hists)
-        for (int e = 0; e < 4; ++e) bar_wait(B(kH + e), (hists - 1) & 1u);
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) wait_for(B(kH + e), (hists - 1) & 1u);
     }
     __syncwarp();
   } else if (warp == kScrubWarp) {
     // ----------------------------------------------------------- V scrub
     uint32_t vt = 0;
+#pragma unroll 1
     for (int i = first; i < last && ok; ++i) {
       const PackedItem& it = a.items[i];
       const int n = (max(it.steps0, it.steps1) + 1) / 2, lo_vis = it.lo_vis, hi_vis = it.hi_vis;
+#pragma unroll 1
       for (int t = 0; t < n; ++t, ++vt) {
         const uint32_t st = vt % NST;
-        if (!__all_sync(0xFFFFFFFFu, bar_wait(B(kVf + st), (vt / NST) & 1u))) {
+        if (!__all_sync(0xFFFFFFFFu, wait_for(B(kVf + st), (vt / NST) & 1u))) {
           fail();
           break;
         }
@@ -441,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 0; x < DP / 64; ++x, tile += HALF_BYTES) {
             uint4* p = reinterpret_cast<uint4*>(tile);  // 8 chunks of 16 bytes per row, swizzled within the row
             uint32_t top = 0u;
+#pragma unroll 4
             for (int c = 8 * lo + lane; c < 8 * hi; c += 32) {
               const uint4 v = p[c];
               top = __vmaxu2(__vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
@@ -449,12 +477,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool bad = max(top & 0xFFFFu, top >> 16) >= kNonFinite<DT>;
             if (__any_sync(0xFFFFFFFFu, bad)) {
               *dirty_flag = 1u;
+#pragma unroll 1
               for (int c = 8 * lo + lane; c < 8 * hi; c += 32) {
                 const uint4 v = p[c];
                 p[c] = make_uint4(v.x & ~nonfinite_mask<DT>(v.x), v.y & ~nonfinite_mask<DT>(v.y),
                                   v.z & ~nonfinite_mask<DT>(v.z), v.w & ~nonfinite_mask<DT>(v.w));
               }
             }
+#pragma unroll 1
             for (int c = 8 * hi + lane; c < 8 * PK; c += 32) p[c] = make_uint4(0u, 0u, 0u, 0u);
           }
           fence_async_smem();
@@ -473,6 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // phases so far, one bit each: the score buffers (0, 1), the last PV and
     // the one before (2, 3), the history (4); V tiles modulo the ring (5, 6)
     uint32_t bits = 0;
+#pragma unroll 1
     for (int i = first; i < last && ok; ++i) {
       int nh, lim;  // the half's steps; the row's visible keys, from the item's first tile
       bool idle;    // no row of the warp's: it only hands its part of P over
@@ -503,13 +534,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       // votes keep the warp together for the TMEM accesses
       auto scores_full = [&](int u, bool tried) {
         if (__all_sync(0xFFFFFFFFu, tried)) return true;
-        const bool r = __all_sync(0xFFFFFFFFu, bar_wait(B(kS + 2 * hf + (u & 1)), s_phase(u)));
+        const bool r = __all_sync(0xFFFFFFFFu, wait_for(B(kS + 2 * hf + (u & 1)), s_phase(u)));
         if (!r) fail();
         return r;
       };
       bool before_seen = false;  // the last PV but one of this item
+#pragma unroll 1
       for (int u = 0; idle && u < nh && scores_full(u, false); ++u) arrive_lane0(B(kP + 2 * hf + (u & 1)), lane);
       if (!idle && nh > 0 && scores_full(0, false)) request(0);
+#pragma unroll 1
       for (int u = 0; !idle && u < nh && ok; ++u) {
         const int buf = u & 1;
         tmem_load_wait();
@@ -568,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // O_h's rows rescaled between PV_h(u - 1), which was issued before
           // S_h(u + 1) and so is over, and PV_h(u), which waits for P_h(u)
           if (!next) {
-            if (!__all_sync(0xFFFFFFFFu, bar_wait(B(kPv + 2 * hf), (bits >> 3) & 1u))) {
+            if (!__all_sync(0xFFFFFFFFu, wait_for(B(kPv + 2 * hf), (bits >> 3) & 1u))) {
               fail();
               break;
             }
@@ -595,8 +628,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       bits ^= uint32_t((nh + 1) / 2) & 1u;
       bits ^= (uint32_t(nh / 2) & 1u) << 1;
       if (ok && nh > 0) {
-        bool r = nh < 2 || before_seen || bar_wait(B(kPv + 2 * hf), (bits >> 3) & 1u);
-        r = bar_wait(B(kPv + 2 * hf + 1), (bits >> 2) & 1u) && r;
+        bool r = nh < 2 || before_seen || wait_for(B(kPv + 2 * hf), (bits >> 3) & 1u);
+        r = wait_for(B(kPv + 2 * hf + 1), (bits >> 2) & 1u) && r;
         if (!__all_sync(0xFFFFFFFFu, r)) fail();
         bits ^= nh > 1 ? 12u : 4u;
         tc_after();
@@ -664,6 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (slow && have) {
           // the zeroed values of keys that this row does see
           const int hi = min(lim, nh * SK);
+#pragma unroll 1
           for (int k = it.lo_vis; k < hi; ++k) {
             const uint16_t* vr = a.v + (int64_t(it.k_start) + it.t_lo * PK + k) * a.v_token +
                                  int64_t(it.kvh) * a.v_head + c0;
@@ -680,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (hist) {
           constexpr int kCols = DP / 2;  // columns per history slot
           const int e = c0 / kCols;
-          if (c0 % kCols == 0 && !__all_sync(0xFFFFFFFFu, bar_wait(B(kH + 2 * hf + e), (bits >> 4) & 1u))) {
+          if (c0 % kCols == 0 && !__all_sync(0xFFFFFFFFu, wait_for(B(kH + 2 * hf + e), (bits >> 4) & 1u))) {
             fail();
             break;
           }
