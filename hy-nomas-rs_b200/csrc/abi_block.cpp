@@ -125,6 +125,9 @@ Lens check_lens(const uint64_t* q_lens, const uint64_t* k_lens, uint64_t n, int3
   // packed rows (tokens x group) and tile coordinates are 32-bit
   constexpr uint64_t kMax = (uint64_t(1) << 31) - 1024;
   const uint64_t group = uint64_t(heads / kv_heads);
+  constexpr uint64_t kMaxItems = uint64_t(1) << 22;  // a quarter of a gigabyte of work list
+  const uint64_t half = group * (nkv::kPackedHalfRows / group);
+  uint64_t items = 0;
   Lens l;
   for (uint64_t s = 0; s < n; ++s) {
     if (q_lens[s] > kMax || k_lens[s] > kMax) fail(NKV_ERR_GEOMETRY, "sequence too long");
@@ -132,6 +135,8 @@ Lens check_lens(const uint64_t* q_lens, const uint64_t* k_lens, uint64_t n, int3
     l.k_tokens += k_lens[s];
     if (l.q_tokens * group > kMax || l.k_tokens > kMax)
       fail(NKV_ERR_GEOMETRY, "packed tokens x heads per group, and packed keys, must be below 2^31");
+    items += (q_lens[s] * group + half - 1) / half * uint64_t(kv_heads);
+    if (items > kMaxItems) fail(NKV_ERR_GEOMETRY, "too many rows for one plan: at most 2^22 work items");
     l.q.push_back(int64_t(q_lens[s]));
     l.k.push_back(int64_t(k_lens[s]));
   }

@@ -309,6 +309,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       // the first PV overwrites O, which the last item's output is read from
       if (i > first && !wait(kOf + hf, item_ph ^ 1u)) break;
+      // a half without steps has its "last PV" here: its softmax warps, which
+      // wait for nothing else, must not free O twice before the wait above
+      if (nh == 0 && elect_one()) mma_commit(B(kPv + 2 * hf + 1));
+      __syncwarp();
       // One round per tile; this half may need fewer steps than the other, but
       // returns every stage to the rings.
 #pragma unroll 1
@@ -627,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const PackedItem it = read_item(a.items + i);
       bits ^= uint32_t((nh + 1) / 2) & 1u;
       bits ^= (uint32_t(nh / 2) & 1u) << 1;
-      if (ok && nh > 0) {
+      if (ok) {
         bool r = nh < 2 || before_seen || wait_for(B(kPv + 2 * hf), (bits >> 3) & 1u);
         r = wait_for(B(kPv + 2 * hf + 1), (bits >> 2) & 1u) && r;
         if (!__all_sync(0xFFFFFFFFu, r)) fail();

@@ -96,6 +96,11 @@ class _Elsewhere:
         self.device.__exit__(None, None, None)
 
 
+def _check_eps(eps) -> None:
+    if not 0.0 <= eps <= 3.4e38:
+        raise ArgumentError("eps must be finite and not negative")
+
+
 def _fresh(like):
     """A contiguous tensor of like's shape and type (empty_like is the quicker
     call, but keeps the strides of a dense one)."""
@@ -264,6 +269,7 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
         raise GeometryError(f"k must be ({tokens}, kv_heads, {D}) {q.dtype}")
     if not norm and (q_weight is not None or k_weight is not None):
         raise ArgumentError("q_weight and k_weight need norm=True")
+    _check_eps(eps)
     pcode = _positions(positions, axes, tokens)
     q_st = q.stride()
     k_st = (0, 0, 1) if k is None else k.stride()
@@ -348,6 +354,7 @@ def residual_norm(x, branch=None, *, gate=None, post=None, post_weight=None, nor
         raise ArgumentError("weight, scale, shift and y_out need a norm")
     if branch is None and not norm_c:
         raise ArgumentError("nothing to do: no branch and no norm")
+    _check_eps(eps)
     wdt = _vector(post_weight, "post_weight", dim, x.dtype, None)
     wdt = _vector(weight, "weight", dim, x.dtype, wdt)
     mdt, groups = None, 0
@@ -410,8 +417,8 @@ def _lens(v: Sequence[int], name: str):
 class AttendPlan:
     """The work list of attend_packed for one set of sequence lengths
     (nkv_attend_plan_create): q_lens query tokens over k_lens keys each
-    (default: the same), `heads` query heads in groups over kv_heads (default:
-    heads) key/value heads, head_dim a multiple of 8 up to 128.  causal: token
+    (default: the same), `heads` query heads in groups of at most 128 over
+    kv_heads (default: heads) key/value heads, head_dim a multiple of 8 up to 128.  causal: token
     i sees the keys up to its own position, aligned to the sequence's last
     key; block > 1: up to the end of the block of `block` keys that holds it
     (tokens per frame: frame-causal).  causal False: every key.
@@ -491,6 +498,10 @@ def attend_packed(plan: AttendPlan, q, k, v, scale: Optional[float] = None, hist
     if q.dim() != 3 or q.shape[1:] != (H, D) or q.shape[0] < plan.q_tokens:
         raise GeometryError(f"q must be (at least {plan.q_tokens}, {H}, {D})")
     rows = q.shape[0]
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    elif not 0.0 < scale <= 3.4e38:
+        raise ArgumentError("scale must be finite and positive")
     for name, t in (("k", k), ("v", v)):
         if t.dim() != 3 or t.shape[1:] != (KV, D) or t.shape[0] < plan.k_tokens or t.dtype != q.dtype:
             raise GeometryError(f"{name} must be (at least {plan.k_tokens}, {KV}, {D}) {q.dtype}")
@@ -537,7 +548,7 @@ def attend_packed(plan: AttendPlan, q, k, v, scale: Optional[float] = None, hist
         (qp, qt, qh), (kp, kt, kh), (vp, vt, vh) = where
         _check(lib().nkv_attend_packed(
             plan._h, _ATTEND.pack(_CODES[q.dtype], _CODES[out.dtype], rows, k_rows, qp, kp, vp, qt, qh, kt, kh, vt, vh,
-                                  1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(), lse.data_ptr(),
+                                  scale, out.data_ptr(), lse.data_ptr(),
                                   ho_p, hl_p, ws.data_ptr() if n else 0, n), _raw_stream(index)))
     finally:
         if away is not None:

@@ -533,8 +533,8 @@ int nkv_residual_norm(const nkv_residual_norm_args* args, void* stream);
 
 /* Packed attention: n sequences, q_lens[s] query tokens over k_lens[s] keys
  * each (0 allowed), packed one after another; `heads` query heads in groups
- * of heads / kv_heads per key/value head (query head h reads key/value head
- * h / (heads / kv_heads)).  Key j is visible to token i of its sequence iff
+ * of heads / kv_heads, at most 128, per key/value head (query head h reads
+ * key/value head h / (heads / kv_heads)).  Key j is visible to token i of its sequence iff
  * j < lim(i): k_len when causal is 0; else ((i + k_len - q_len) / block + 1) *
  * block, at most k_len, and 0 when i + k_len - q_len < 0 (block 1: ordinary
  * causal, aligned to the last token; block = tokens per frame: a token sees

@@ -81,6 +81,8 @@ def test_schedule_fills_the_gpu_for_one_token(nkv):
     ([1], [1], 4, -4, 1, "GeometryError"), ([1], [1], 4, 4, 0, "ArgumentError"), ([2 ** 31], [1], 1, 1, 1, "GeometryError"),
     ([2 ** 63], [2 ** 63], 1, 1, 1, "GeometryError"), ([2 ** 30], [1], 4, 1, 1, "GeometryError"),
     ([1, 1], [2 ** 30, 2 ** 30], 1, 1, 1, "GeometryError"), ([1], [1], 4, 4, 2 ** 31, "ArgumentError"),
+    ([1], [1], 129, 1, 1, "GeometryError"), ([2 ** 28], [1], 8, 8, 1, "GeometryError"),
+    ([1] * 70, [1] * 70, 65535, 65535, 1, "GeometryError"),
 ])
 def test_schedule_and_plan_refuse_bad_geometry(nkv, q, k, heads, kv, block, code):
     with pytest.raises(getattr(nkv, code)):

@@ -130,6 +130,14 @@ CASES = [
     ([2, 1, 300], [5000, 33, 12000], 4, 4, 128, True, 1),
     ([2100], [2100], 2, 2, 64, True, 1),
     ([0, 0], [0, 3], 2, 2, 64, True, 1),
+    ([9], [300], 128, 1, 64, True, 1),                           # the largest group
+    ([9], [300], 127, 1, 64, True, 1),                           # one token per half of an item
+    ([70], [70], 48, 2, 128, True, 1),                           # groups of 24: 120 of 128 rows
+    ([1] * 40, list(range(0, 400, 10)), 4, 2, 128, True, 1),     # many single tokens
+    ([1, 2, 3] * 20, [500] * 60, 3, 3, 48, False, 1),            # several items of one half on a CTA
+    ([1] * 400, [3] * 400, 2, 2, 64, True, 1),
+    ([1] * 300, [0, 5, 0, 0, 200, 0] * 50, 4, 4, 128, True, 1),  # and items without keys among them
+    ([130, 1, 0, 2] * 60, [130, 0, 4, 70] * 60, 3, 3, 64, True, 1),
 ]
 
 
@@ -145,6 +153,56 @@ def test_matches_float64(nkv, case, dtype):
     plan.check()
     assert out.dtype == q.dtype and out.shape == q.shape and lse.shape == (H, q.shape[0])
     _check(q, k, v, ql, kl, out, lse, causal, block)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_geometry(nkv, seed):
+    """Lengths, groups, widths, masks, history and layouts drawn together."""
+    import random
+
+    import torch
+    rng = random.Random(seed)
+    n = rng.choice([1, 1, 2, 4, 7])
+    pick = lambda hi: max(0, int(math.exp(rng.uniform(0, math.log(hi)))) - rng.choice([0, 0, 1]))  # noqa: E731
+    ql = [pick(rng.choice([3, 60, 900])) for _ in range(n)]
+    kl = [q if rng.random() < 0.4 else max(0, q + rng.choice([-5, 1, 64, 1000, 7000])) for q in ql]
+    KV = rng.choice([1, 2, 3, 5])
+    H = KV * rng.choice([1, 2, 3, 6, 8])
+    D = rng.choice([64, 128, 8 * rng.randint(1, 16)])
+    causal, block = rng.random() < 0.8, rng.choice([1, 1, 30, 400])
+    dt = rng.choice([torch.bfloat16, torch.float16])
+    q, k, v = _inputs(ql, kl, H, KV, D, dt, seed=seed, qs=rng.choice([0.5, 1.0, 4.0]))
+    if rng.random() < 0.5:  # one projection's views
+        kv = torch.cat((k, v), dim=1)
+        k, v = kv[:, :KV], kv[:, KV:]
+    history = None
+    if rng.random() < 0.4:
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        history = (torch.randn(q.shape, generator=g, device="cuda"),
+                   6 * torch.rand((H, q.shape[0]), generator=g, device="cuda"))
+    plan = nkv.AttendPlan(ql, H, kv_heads=KV, head_dim=D, k_lens=kl, causal=causal, block=block)
+    out = torch.empty(q.shape, dtype=torch.float32, device="cuda") if rng.random() < 0.3 else None
+    out, lse = nkv.attend_packed(plan, q, k, v, history=history, out=out)
+    plan.check()
+    _check(q, k, v, ql, kl, out, lse, causal, block, history=history)
+
+
+def test_offsets_past_32_bits(nkv):
+    """Keys, values and queries as columns of buffers whose rows lie half a megabyte apart."""
+    import torch
+    T, W = 9000, 1 << 18
+    q, k, v = _inputs([T], [T], 1, 1, 64, torch.bfloat16, seed=11)
+    buf = torch.empty((T, 1, W), dtype=torch.bfloat16, device="cuda")  # 4.7 GB
+    wide = [buf[..., c:c + 64] for c in (0, W // 2, W - 64)]
+    for w, t in zip(wide, (q, k, v)):
+        w.copy_(t)
+    last = slice(T - 300, T)
+    plan = nkv.AttendPlan([T], 1, head_dim=64)
+    out, lse = nkv.attend_packed(plan, *wide)
+    near, near_lse = nkv.attend_packed(plan, q, k, v)
+    assert torch.equal(out, near) and torch.equal(lse, near_lse)
+    _check(q[last], k, v, [300], [T], out[last], lse[:, last])
+    del buf
 
 
 def test_f32_output_and_scale(nkv):
@@ -330,7 +388,7 @@ def test_refusals(nkv):
     bad = [
         (ge, dict(q=q[:3])), (ge, dict(q=q[:, :2])), (ge, dict(q=q.float())), (ge, dict(k=k[:7])),
         (ge, dict(k=k.half())), (ge, dict(v=v[:, :1])), (ge, dict(q=q.transpose(1, 2).contiguous().transpose(1, 2))),
-        (ae, dict(scale=0.0)), (ae, dict(scale=-1.0)), (ae, dict(scale=math.inf)), (ae, dict(scale=math.nan)),
+        (ae, dict(scale=0.0)), (ae, dict(scale=-1.0)), (ae, dict(scale=1e60)), (ae, dict(scale=1e-60)), (ae, dict(scale=math.inf)), (ae, dict(scale=math.nan)),
         (ae, dict(q=q.clone().requires_grad_())), (ae, dict(k=k.cpu())),
         (ge, dict(out=torch.empty((4, 4, 64), dtype=torch.float16, device="cuda"))),
         (ge, dict(out=torch.empty((3, 4, 64), dtype=torch.bfloat16, device="cuda"))),

@@ -166,6 +166,21 @@ def test_strides_and_in_place(nkv, dim):
     _check(rows, a["b"], nkv.residual_norm(rows, a["b"], **kw), **kw)
 
 
+@pytest.mark.parametrize("dim", [256, 255])
+def test_offsets_past_32_bits(nkv, dim):
+    import torch
+    T, W = 9000, 1 << 18
+    a = _make(T, dim, torch.bfloat16, 4, torch.float32)
+    buf = torch.empty((T, W), dtype=torch.bfloat16, device="cuda")  # 4.7 GB
+    x, b = buf[:, :dim], buf[:, W - 256:W - 256 + dim]
+    x.copy_(a["x"])
+    b.copy_(a["b"])
+    kw = dict(gate=a["gate"], scale=a["scale"], shift=a["shift"], mod_index=a["mod_index"], post="rms")
+    want = nkv.residual_norm(a["x"], a["b"], **kw)
+    got = nkv.residual_norm(x, b, h_out=x, y_out=b, **kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_graph_and_other_stream(nkv):
     import torch
     a = _make(100, 512, torch.bfloat16, 1, torch.float32)
@@ -201,7 +216,7 @@ def test_refusals(nkv):
         (ge, dict(scale=m, mod_index=idx.long())), (ae, dict(mod_index=idx)), (ge, dict(weight=v[:32])),
         (ge, dict(weight=v.half())), (ge, dict(branch=b, weight=v, post="rms", post_weight=v.bfloat16())),
         (ge, dict(y_out=x.float())), (ge, dict(h_out=x[:3], branch=b)), (ae, dict(h_out=x)),
-        (ae, dict(branch=b, h_out=x, y_out=x)), (ae, dict(eps=-1.0)), (ae, dict(eps=math.nan)),
+        (ae, dict(branch=b, h_out=x, y_out=x)), (ae, dict(eps=-1.0)), (ae, dict(eps=math.nan)), (ae, dict(eps=1e60)),
         (ae, dict(x=x.float().requires_grad_())), (ae, dict(weight=v.cpu())),
     ]:
         a = dict(x=x)

@@ -171,6 +171,24 @@ def test_nonfinite_values_stay_in_their_pairs(nkv):
     assert bad.nonzero().tolist() == [[2, 1, 4], [2, 1, 5]]
 
 
+def test_offsets_past_32_bits(nkv):
+    import torch
+    T, W = 9000, 1 << 18
+    buf = torch.empty((T, 1, W), dtype=torch.bfloat16, device="cuda")  # 4.7 GB
+    q, k = torch.randn((T, 1, 128), device="cuda").bfloat16(), torch.randn((T, 1, 128), device="cuda").bfloat16()
+    qw, kw = buf[..., :128], buf[..., W - 128:]
+    qw.copy_(q)
+    kw.copy_(k)
+    pos, axes = _pos(T, 3, "int32"), nkv.RotaryAxes((44, 42, 42))
+    want = nkv.rotary(pos, axes, q, k=k, norm=True)
+    got = nkv.rotary(pos, axes, qw, k=kw, norm=True, q_out=qw, k_out=kw)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    odd = nkv.RotaryAxes((36, 2))
+    want = nkv.rotary(pos[:, :2].contiguous(), odd, q[..., :44].contiguous())  # the path for any head_dim
+    qw.copy_(q)
+    assert torch.equal(nkv.rotary(pos[:, :2].contiguous(), odd, qw[..., :44]), want)
+
+
 def test_graph_and_other_stream(nkv):
     import torch
     T = 300
@@ -212,7 +230,8 @@ def test_refusals(nkv):
         (ge, dict(q_out=q.float())), (ge, dict(q_out=q[:, :1].expand(4, 2, 64))),
         (ae, dict(q=q[:, :1], q_out=q[:, 1:].clone().as_strided((4, 1, 64), (64, 64, 1)), k=None,
                   positions=pos.cpu())),
-        (ae, dict(q=q.clone().requires_grad_())), (ae, dict(norm=True, eps=-1.0)),
+        (ae, dict(q=q.clone().requires_grad_())), (ae, dict(norm=True, eps=-1.0)), (ae, dict(norm=True, eps=1e60)),
+        (ae, dict(norm=True, eps=math.nan)),
     ]:
         a = dict(positions=pos, axes=ax, q=q)
         a.update(kw)
