@@ -319,6 +319,9 @@ int nkv_attend_plan_create(const uint64_t* q_lens, const uint64_t* k_lens, uint6
                 host.data() + p->units_off);
     cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&p->table), host.size());
     if (e == cudaSuccess) e = cudaMemcpy(p->table, host.data(), host.size(), cudaMemcpyHostToDevice);
+    // a copy from pageable memory may return before it has landed, and the
+    // plan's calls come on streams that do not wait for the default stream
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
       if (p->table) cudaFree(p->table);
       nkv::check_cuda(e, "attention plan upload");
@@ -368,7 +371,9 @@ int nkv_attend_packed(const nkv_attend_plan* plan, const nkv_attend_args* a, voi
       fail(NKV_ERR_GEOMETRY, "packed attention needs bf16 or f16 queries, keys and values");
     if (a->out_dtype != a->dtype && a->out_dtype != NKV_F32)
       fail(NKV_ERR_GEOMETRY, "the output must be f32 or of the queries' type");
-    if (!(a->scale > 0.0f) || !std::isfinite(a->scale)) fail(NKV_ERR_ARGUMENT, "scale must be finite and positive");
+    const float scale_log2 = a->scale * 1.4426950408889634f;
+    if (!(scale_log2 > 0.0f) || !std::isfinite(scale_log2))
+      fail(NKV_ERR_ARGUMENT, "scale must be finite and positive");
     if (a->q_rows < plan->q_tokens || a->k_rows < plan->k_tokens)
       fail(NKV_ERR_GEOMETRY, "q has " + std::to_string(a->q_rows) + " rows and k / v " + std::to_string(a->k_rows) +
                                  ", the plan " + std::to_string(plan->q_tokens) + " and " +
@@ -411,7 +416,7 @@ int nkv_attend_packed(const nkv_attend_plan* plan, const nkv_attend_args* a, voi
     p.hist_o = a->hist_out;
     p.hist_lse = a->hist_lse;
     p.hist_lse_head = int64_t(a->q_rows);
-    p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.scale_log2 = scale_log2;
     p.part_o = static_cast<float*>(a->workspace);
     p.part_ml = p.part_o ? p.part_o + plan->part_rows * uint64_t(plan->D) : nullptr;
     p.status = reinterpret_cast<uint32_t*>(plan->table);

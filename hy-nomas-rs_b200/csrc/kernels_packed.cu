@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (hist && have) {
           const float zh = __ldg(a.hist_lse + int64_t(h) * a.hist_lse_head + q) * 1.4426950408889634f;
           const float M = fmaxf(z, zh);
-          if (M == -INFINITY) {
+          if (z == -INFINITY && zh == -INFINITY) {  // (not M, which forgets a NaN)
             wo = 0.0f;
           } else {
             const float e0 = exp2f(z - M), e1 = exp2f(zh - M), inv = 1.0f / (e0 + e1);

@@ -109,6 +109,8 @@ def _fresh(like):
 
 def _enter(index, stream, tensors):
     """None where the call runs on the current device's current stream."""
+    if stream is not None and stream.device_index != index:
+        raise ArgumentError(f"the stream is on device {stream.device_index}, the tensors on {index}")
     if stream is None and torch.cuda.current_device() == index:
         return None
     return _Elsewhere(index, stream, tensors)
@@ -251,7 +253,7 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
     norm per head with the (D) gains q_weight / k_weight comes first.  D even,
     up to 256; f32, bf16 or f16; any token and head strides with the last
     dimension dense, so q and k may be views of one fused projection.  q_out /
-    k_out may be q / k themselves (in place).  Returns q_out, or (q_out,
+    k_out may be q / k themselves (in place, where k is not q).  Returns q_out, or (q_out,
     k_out) when k is given."""
     index = _device_of(q, k, positions, q_weight, k_weight, q_out, k_out)
     code = _code(q, "q")
@@ -279,10 +281,11 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
         if w is not None and (w.shape != (D,) or w.dtype != q.dtype or not w.is_contiguous()):
             raise GeometryError(f"{name} must be a contiguous ({D},) {q.dtype} tensor")
     ins = (q, k, positions, q_weight, k_weight)
+    apart = k is q  # read as both: neither may be rotated in place
     away = _enter(index, stream, (*ins, q_out, k_out))
     try:
         if q_out is not None:
-            _check_out(q_out, q, ins, "q_out", alias=(q,), others=(k_out,))
+            _check_out(q_out, q, ins, "q_out", alias=() if apart else (q,), others=(k_out,))
             qo_st = q_out.stride()
         else:
             q_out = _fresh(q)
@@ -291,7 +294,7 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
         if k is not None:
             k_heads = k.shape[1]
             if k_out is not None:
-                _check_out(k_out, k, ins, "k_out", alias=(k,), others=(q_out,))
+                _check_out(k_out, k, ins, "k_out", alias=() if apart else (k,), others=(q_out,))
                 ko_st = k_out.stride()
             else:
                 k_out = _fresh(k)

@@ -187,6 +187,27 @@ def test_random_geometry(nkv, seed):
     _check(q, k, v, ql, kl, out, lse, causal, block, history=history)
 
 
+@pytest.mark.parametrize("k_len", [70, 9000])
+def test_nan_rows_stay_nan_in_the_merge(nkv, k_len):
+    """A NaN of either part is not taken for "nothing seen" when the other part saw nothing."""
+    import torch
+    q, k, v = _inputs([70], [k_len], 1, 1, 64, torch.bfloat16)
+    q[3] = math.nan
+    ho, hl = torch.randn((70, 1, 64), device="cuda"), torch.full((1, 70), -math.inf, device="cuda")
+    hl[0, 5] = math.nan
+    plan = nkv.AttendPlan([70], 1, head_dim=64, k_lens=[k_len])
+    out, lse = nkv.attend_packed(plan, q, k, v, history=(ho, hl))
+    bad = torch.zeros(70, dtype=torch.bool, device="cuda")
+    bad[3] = bad[5] = True
+    assert torch.equal(out.isnan().all(-1)[:, 0], bad) and torch.equal(out.isnan().any(-1)[:, 0], bad)
+    assert torch.equal(lse.isnan()[0], bad)
+    none = nkv.AttendPlan([70], 1, head_dim=64, k_lens=[0])
+    out, lse = nkv.attend_packed(none, q, k, v, history=(ho, hl))
+    bad[3] = False
+    assert torch.equal(out.isnan().all(-1)[:, 0], bad) and torch.equal(lse.isnan()[0], bad)
+    assert bool((lse[0, ~bad] == -math.inf).all()) and bool((out[~bad] == 0).all())
+
+
 def test_offsets_past_32_bits(nkv):
     """Keys, values and queries as columns of buffers whose rows lie half a megabyte apart."""
     import torch
@@ -388,7 +409,7 @@ def test_refusals(nkv):
     bad = [
         (ge, dict(q=q[:3])), (ge, dict(q=q[:, :2])), (ge, dict(q=q.float())), (ge, dict(k=k[:7])),
         (ge, dict(k=k.half())), (ge, dict(v=v[:, :1])), (ge, dict(q=q.transpose(1, 2).contiguous().transpose(1, 2))),
-        (ae, dict(scale=0.0)), (ae, dict(scale=-1.0)), (ae, dict(scale=1e60)), (ae, dict(scale=1e-60)), (ae, dict(scale=math.inf)), (ae, dict(scale=math.nan)),
+        (ae, dict(scale=0.0)), (ae, dict(scale=-1.0)), (ae, dict(scale=1e60)), (ae, dict(scale=1e-60)), (ae, dict(scale=3e38)), (ae, dict(scale=math.inf)), (ae, dict(scale=math.nan)),
         (ae, dict(q=q.clone().requires_grad_())), (ae, dict(k=k.cpu())),
         (ge, dict(out=torch.empty((4, 4, 64), dtype=torch.float16, device="cuda"))),
         (ge, dict(out=torch.empty((3, 4, 64), dtype=torch.bfloat16, device="cuda"))),

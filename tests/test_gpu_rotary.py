@@ -9,6 +9,7 @@ r for the table, 3 * 2^-24 r for the products and the sum, and for the norm (D
 / 2 + 8) 2^-24 r for the sum of squares, the root and the products.
 """
 import math
+import types
 
 import pytest
 
@@ -242,6 +243,13 @@ def test_refusals(nkv):
         nkv.rotary(pos, ax, x[:4], q_out=x[1:])
     with pytest.raises(ae, match="overlaps"):
         nkv.rotary(pos, ax, q, k=x[:4], q_out=x[:4])
+    for kw in (dict(q_out=q), dict(k_out=q), dict(q_out=q, k_out=q)):  # one tensor read as both
+        with pytest.raises(ae, match="overlaps"):
+            nkv.rotary(pos, ax, q, k=q, **kw)
+    one, two = nkv.rotary(pos, ax, q, k=q)
+    assert torch.equal(one, two)
+    with pytest.raises(ae, match="stream"):
+        nkv.rotary(pos, ax, q, stream=types.SimpleNamespace(device_index=1, cuda_stream=0))
     with pytest.raises(ae, match="overlaps"):
         t = torch.empty((4, 32), device="cuda")
         nkv.rope_tables(pos, ax, cos=t, sin=t)
