@@ -18,7 +18,9 @@
 // would cost more than the row itself.  That leaves room for two CTAs an SM at
 // 5,120 columns, too few loads in flight for HBM if they went to registers as
 // well: rows arrive by cp.async, several ahead, each thread waiting for its own
-// bytes only.
+// bytes only.  Measured: 6,496 rows of 5,120 bf16 columns with norms on both
+// sides and five modulation groups (266 MB): 54 us, 4.9 TB/s, where a plain
+// copy of as many bytes takes 47.  One row: 5 us, a launch.
 #include <algorithm>
 
 #include "nkv_device.cuh"
@@ -187,6 +189,12 @@ __device__ __forceinline__ void products8(const ResidualNormParams& a, int g, in
 // dim a multiple of 8 up to 8192, everything 16-byte aligned: thread j of the
 // CTA owns the 8-column chunks j and j + threads, and in shared memory the
 // bytes of its chunks of the kAhead rows on their way.
+//
+// 96 registers a thread, so that two CTAs of 320 threads share an SM (at 100
+// one does: 108 us for the 266 MB above, against 87 then).  The instructions
+// count next: addresses that advance row by row, and x unpacked only when the
+// branch's norm is known, took 583 instructions per row and warp to 427 and
+// 61 us to 54 (8,192 columns: 94 to 75).
 template <int DT, int kAhead>
 __global__ void __maxnreg__(96) k_residual_norm_vec(const ResidualNormParams a) {
   extern __shared__ uint4 ring[];
@@ -200,92 +208,114 @@ __global__ void __maxnreg__(96) k_residual_norm_vec(const ResidualNormParams a) 
   const float inv_dim = 1.0f / float(a.dim);
   const uint64_t r0 = uint64_t(blockIdx.x) * a.rows_per_cta;
   const int rows = int(min(a.tokens - r0, a.rows_per_cta));
-  // piece p of chunk k of x (0) or branch (1) in ring row `row`
-  auto piece = [&](int row, int tensor, int k, int p) {
-    return ring + ((row * 2 + tensor) * kPieces + p) * chunks + c0 + k * threads;
+  // Every address advances by a row at a time; in a row of the ring x comes
+  // before the branch, a chunk's pieces `chunks` apart.
+  auto first = [&](const void* base, int64_t stride) {
+    return reinterpret_cast<uintptr_t>(base) + uintptr_t((int64_t(r0) * stride + 8 * c0) * kSize);
   };
-  auto request = [&](int r, int row) {
-    if (r < rows) {
+  uintptr_t x_src = first(a.x, a.x_stride), b_src = first(a.branch, a.branch_stride);
+  uintptr_t h_dst = first(a.h_out, a.h_stride), y_dst = first(a.y_out, a.y_stride);
+  const int gap = 8 * threads * kSize;  // bytes to the second chunk in a row of a tensor; in the ring:
+  const uint32_t ring_gap = uint32_t(threads) * 16u, ring_piece = uint32_t(chunks) * 16u,
+                 ring_row = 2u * kPieces * ring_piece;
+  const uint32_t ring0 = static_cast<uint32_t>(__cvta_generic_to_shared(ring + c0));
+  const uint32_t ring_end = ring0 + kAhead * ring_row;
+  auto copy = [&](uint32_t dst, uintptr_t src) {
 #pragma unroll
-      for (int tensor = 0; tensor < 2; ++tensor) {
-        const void* src = tensor ? a.branch : a.x;
-        if (!src) continue;
-        const unsigned char* q = static_cast<const unsigned char*>(src) +
-                                 ((int64_t(r0) + r) * (tensor ? a.branch_stride : a.x_stride) + 8 * c0) * kSize;
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int p = 0; p < kPieces; ++p)
-            if (have[k])
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(
-                               __cvta_generic_to_shared(piece(row, tensor, k, p)))),
-                           "l"(q + 8 * k * threads * kSize + 16 * p)
-                           : "memory");
+      for (int p = 0; p < kPieces; ++p)
+        if (have[k])
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + uint32_t(k) * ring_gap +
+                                                                        uint32_t(p) * ring_piece),
+                       "l"(src + (k ? gap : 0) + 16 * p)
+                       : "memory");
+  };
+  int left = rows;  // rows not asked for yet
+  auto request = [&](uint32_t at) {
+    if (left-- > 0) {
+      copy(at, x_src);
+      x_src += uintptr_t(a.x_stride * kSize);
+      if (a.branch) {
+        copy(at + kPieces * ring_piece, b_src);
+        b_src += uintptr_t(a.branch_stride * kSize);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto arrived = [&](int row, int tensor, int k, float* x) {
+  auto arrived = [&](uint32_t at, int k, float* x) {  // chunk k; absent: zeros
     Raw8<DT> raw;
 #pragma unroll
-    for (int p = 0; p < kPieces; ++p) raw.w[p] = *piece(row, tensor, k, p);
+    for (int p = 0; p < kPieces; ++p) {
+      raw.w[p] = make_uint4(0u, 0u, 0u, 0u);
+      if (have[k])
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(raw.w[p].x), "=r"(raw.w[p].y), "=r"(raw.w[p].z), "=r"(raw.w[p].w)
+                     : "r"(at + uint32_t(k) * ring_gap + uint32_t(p) * ring_piece)
+                     : "memory");
+    }
     unpack_row8<DT>(raw, x);
   };
+  // v * inv * P + Q of 8 values, on packed pairs
+  auto scaled = [](const float* v, float inv, const float* P, const float* Q, float* out) {
 #pragma unroll
-  for (int d = 0; d < kAhead; ++d) request(d, d);
-  int next_group = group_of(a, r0), group = -2, row = 0;
+    for (int j = 0; j < 8; j += 2) {
+      const float2 u = __ffma2_rn(__fmul2_rn(make_float2(v[j], v[j + 1]), make_float2(inv, inv)),
+                                  make_float2(P[j], P[j + 1]), make_float2(Q[j], Q[j + 1]));
+      out[j] = u.x, out[j + 1] = u.y;
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) request(ring0 + uint32_t(d) * ring_row);
+  uint32_t at = ring0;
+  const int32_t* index = a.mod_index ? a.mod_index + r0 : nullptr;
+  int next_group = group_of(a, r0), group = -2;
   float G[16], W[16], S[16];
-  for (int r = 0; r < rows; ++r) {
-    const int g = next_group;
-    if (r + 1 < rows) next_group = group_of(a, r0 + uint64_t(r) + 1);
-    if (g != group) {
-      group = g;
+#pragma unroll 1
+  for (int r = rows; r > 0; --r) {
+    if (next_group != group) {
+      group = next_group;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (have[k]) products8<DT>(a, g, 8 * int64_t(c0 + k * threads), G + 8 * k, W + 8 * k, S + 8 * k);
+        if (have[k]) products8<DT>(a, group, 8 * int64_t(c0 + k * threads), G + 8 * k, W + 8 * k, S + 8 * k);
+    }
+    if (index && r > 1) {
+      next_group = __ldg(++index);
+      if (uint32_t(next_group) >= uint32_t(a.mod_rows)) next_group = -1;
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
-    float h[16], b[16];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (have[k]) {
-        arrived(row, 0, k, h + 8 * k);
-        if (a.branch) arrived(row, 1, k, b + 8 * k);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[8 * k + j] = b[8 * k + j] = 0.0f;
-      }
-    }
-    request(r + kAhead, row);
-    if (++row == kAhead) row = 0;
-    // v = v * inv * P + Q on packed pairs
-    auto scaled = [](const float* v, float inv, const float* P, const float* Q, float* out) {
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float2 u = __ffma2_rn(__fmul2_rn(make_float2(v[j], v[j + 1]), make_float2(inv, inv)),
-                                    make_float2(P[j], P[j + 1]), make_float2(Q[j], Q[j + 1]));
-        out[j] = u.x, out[j + 1] = u.y;
-      }
-    };
-    const int64_t t = int64_t(r0) + r;
+    float h[16];  // the branch, then the stream
     if (a.branch) {
-      const float inv = a.post ? normalise(b, n, inv_dim, a.eps, a.post, part, slot) : 1.0f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) arrived(at + kPieces * ring_piece, k, h + 8 * k);
+      const float inv = a.post ? normalise(h, n, inv_dim, a.eps, a.post, part, slot) : 1.0f;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if (!have[k]) continue;
-        scaled(b + 8 * k, inv, G + 8 * k, h + 8 * k, h + 8 * k);
-        store_row8<DT>(a.h_out, t * a.h_stride + 8 * (c0 + k * threads), h + 8 * k);
+        float x[8];
+        arrived(at, k, x);
+        scaled(h + 8 * k, inv, G + 8 * k, x, h + 8 * k);
+        if (have[k]) store_row8<DT>(reinterpret_cast<void*>(h_dst + (k ? gap : 0)), 0, h + 8 * k);
+        else
+#pragma unroll
+          for (int j = 0; j < 8; ++j) h[8 * k + j] = 0.0f;
       }
+      h_dst += uintptr_t(a.h_stride * kSize);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) arrived(at, k, h + 8 * k);
     }
+    request(at);
+    at += ring_row;
+    if (at == ring_end) at = ring0;
     if (a.norm) {
       const float inv = normalise(h, n, inv_dim, a.eps, a.norm, part, slot);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if (!have[k]) continue;
         float y[8];
         scaled(h + 8 * k, inv, W + 8 * k, S + 8 * k, y);
-        store_row8<DT>(a.y_out, t * a.y_stride + 8 * (c0 + k * threads), y);
+        if (have[k]) store_row8<DT>(reinterpret_cast<void*>(y_dst + (k ? gap : 0)), 0, y);
       }
+      y_dst += uintptr_t(a.y_stride * kSize);
     }
   }
 }
@@ -311,7 +341,9 @@ __device__ __forceinline__ void put_row(void* p, int64_t base, int n, int thread
     if (k < n) put<DT>(p, at + k * threads, v[k]);
 }
 
-// Any dim and any alignment: blockDim.x threads per row, each holding the E
+// Any dim and any alignment (what k_residual_norm_vec cannot take: where both
+// can, 6,496 rows of 5,120 columns take 152 us here, 52 there; of 128 columns 9
+// and 8): blockDim.x threads per row, each holding the E
 // values tid, tid + blockDim.x, ...; one row per CTA, or one per warp when 32
 // threads suffice.
 template <int DT, int E, int kMaxThreads>
