@@ -27,8 +27,9 @@ struct nkv_attend_plan {
   int64_t block = 1;
   uint64_t q_tokens = 0, k_tokens = 0, part_rows = 0;
   int32_t n_items = 0, n_ctas = 0, n_units = 0, max_unit_rows = 0;
-  unsigned char* table = nullptr;  // status word (64 bytes), items, CTAs' first items, units
-  size_t items_off = 64, ctas_off = 0, units_off = 0;
+  // status word (64 bytes), items, where each CTA's begin, each one's first, units
+  unsigned char* table = nullptr;
+  size_t items_off = 64, ctas_off = 0, first_off = 0, units_off = 0;
   uint64_t workspace() const {  // partial rows, then their (max, sum)
     return part_rows * (uint64_t(D) * sizeof(float) + sizeof(float2));
   }
@@ -309,12 +310,16 @@ int nkv_attend_plan_create(const uint64_t* q_lens, const uint64_t* k_lens, uint6
     p->max_unit_rows = s.max_unit_rows;
     auto after = [](size_t at, size_t bytes) { return (at + bytes + 63) / 64 * 64; };
     p->ctas_off = after(p->items_off, s.items.size() * sizeof(nkv::PackedItem));
-    p->units_off = after(p->ctas_off, s.cta_begin.size() * sizeof(int32_t));
+    p->first_off = after(p->ctas_off, s.cta_begin.size() * sizeof(int32_t));
+    p->units_off = after(p->first_off, size_t(p->n_ctas) * sizeof(nkv::PackedItem));
     std::vector<unsigned char> host(after(p->units_off, s.units.size() * sizeof(nkv::PackedUnit)), 0);
     std::copy_n(reinterpret_cast<const unsigned char*>(s.items.data()), s.items.size() * sizeof(nkv::PackedItem),
                 host.data() + p->items_off);
     std::copy_n(reinterpret_cast<const unsigned char*>(s.cta_begin.data()), s.cta_begin.size() * sizeof(int32_t),
                 host.data() + p->ctas_off);
+    for (int32_t c = 0; c < p->n_ctas; ++c)
+      std::copy_n(reinterpret_cast<const unsigned char*>(&s.items[size_t(s.cta_begin[size_t(c)])]),
+                  sizeof(nkv::PackedItem), host.data() + p->first_off + size_t(c) * sizeof(nkv::PackedItem));
     std::copy_n(reinterpret_cast<const unsigned char*>(s.units.data()), s.units.size() * sizeof(nkv::PackedUnit),
                 host.data() + p->units_off);
     cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&p->table), host.size());
@@ -400,6 +405,7 @@ int nkv_attend_packed(const nkv_attend_plan* plan, const nkv_attend_args* a, voi
     nkv::PackedArgs p{};
     p.items = reinterpret_cast<const nkv::PackedItem*>(plan->table + plan->items_off);
     p.units = reinterpret_cast<const nkv::PackedUnit*>(plan->table + plan->units_off);
+    p.first = reinterpret_cast<const nkv::PackedItem*>(plan->table + plan->first_off);
     p.cta_begin = reinterpret_cast<const int32_t*>(plan->table + plan->ctas_off);
     p.n_ctas = plan->n_ctas, p.n_units = plan->n_units, p.max_unit_rows = plan->max_unit_rows;
     p.H = plan->H, p.G = plan->H / plan->kv_heads, p.D = plan->D;

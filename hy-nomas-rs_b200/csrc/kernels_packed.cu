@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile uint32_t* abort_flag = tslot + 1;
   volatile uint32_t* dirty_flag = tslot + 2;  // some V value was zeroed in this CTA
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.launch_dependents;");  // the merge may take SMs that have nothing left to do
   const int G = a.G;
   const int first = a.cta_begin[blockIdx.x], last = a.cta_begin[blockIdx.x + 1];  // this CTA's items
   auto B = [&](int i) { return smem_addr(&bars[i]); };
@@ -232,22 +233,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid == 32 * kTmaWarp) {
+  PackedItem head{};  // the TMA warp's: the first loads wait for one read of the list, not for two in turn
+  if (warp == kTmaWarp) {
+    head = read_item(a.first + blockIdx.x);
+    for (const CUtensorMap* m : {&kmap, &qmap, &vmap})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
     // arrivals per phase: P, O free and history read by the half's 4 warps, K / V empty by both MMA warps, else 1
 #pragma unroll 1
-    for (int i = 0; i < kBarCount; ++i) {
+    for (int i = lane; i < kBarCount; i += 32) {
       const bool by_half = (i >= kP && i < kP + 4) || (i >= kOf && i < kOf + 2) || (i >= kHr && i < kHr + 4);
       const int count = by_half ? 4 : (i >= kKe && i < kKe + NST) || i >= kVe ? 2 : 1;
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(B(i)), "r"(count) : "memory");
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    *abort_flag = 0u;
-    *dirty_flag = 0u;
+    fence_async_smem();
+    if (lane == 0) *abort_flag = *dirty_flag = 0u;
   }
-  tc_before();
-  __syncthreads();
-  tc_after();
-  const uint32_t tmem = *tslot;
+  // The barriers and flags are the TMA warp's, which needs nothing of the
+  // others': it only announces them and goes on to its loads.
+  uint32_t tmem = 0u;
+  if (warp == kTmaWarp) {
+    __syncwarp();
+    asm volatile("bar.arrive 1, %0;" ::"n"(kThreads) : "memory");
+  } else {
+    tc_before();
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+    tc_after();
+    tmem = *tslot;
+  }
   bool ok = true;
   auto fail = [&]() {
     *abort_flag = 1u;
@@ -386,8 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // Q of item i: the box is the group's heads by half_rows / G tokens; rows
       // behind the sequence belong to rows that are not kept
-      auto load_q = [&](int i) {
-        const PackedItem& it = a.items[i];
+      auto load_q = [&](int i, const PackedItem& it) {
 #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
           if (i > first && !wait(kQe + hf, uint32_t(i - first - 1) & 1u)) return false;
@@ -418,19 +430,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       auto tiles_of = [&](const PackedItem& it) { return (max(it.steps0, it.steps1) + 1) / 2; };
       if (first < last) {
-        if (tiles_of(a.items[first]) > 0) load_k(a.items[first], 0);
-        load_q(first);
+        if (tiles_of(head) > 0) load_k(head, 0);
+        load_q(first, head);
       }
       int qs = first < last ? 1 : 0;
-  #pragma unroll 1
+#pragma unroll 1
     for (int i = first; i < last && ok; ++i) {
-        const PackedItem it = a.items[i];
+        const PackedItem it = i == first ? head : read_item(a.items + i);
         const int n = tiles_of(it);
         bool run = true;
 #pragma unroll 1
         for (int t = 0; t < n && run; ++t) run = load_v(it, t) && (t + 1 == n || load_k(it, t + 1));
         if (run && i + 1 < last) {
-          run = (tiles_of(a.items[i + 1]) == 0 || load_k(a.items[i + 1], 0)) && load_q(i + 1);
+          const PackedItem up = read_item(a.items + i + 1);
+          run = (tiles_of(up) == 0 || load_k(up, 0)) && load_q(i + 1, up);
           qs += run;
         }
         if (run && a.hist_o && it.part_row < 0) run = load_history(it);
@@ -780,44 +793,67 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // The merge of a split unit's partial rows (and the history part), one warp
 // per row: with M the largest maximum, o = sum_p 2^(m_p - M) O_p / L,
-// L = sum_p 2^(m_p - M) l_p, lse = (M + log2 L) ln 2.
+// L = sum_p 2^(m_p - M) l_p, lse = (M + log2 L) ln 2.  It moves a few hundred
+// kilobytes, so what counts is how many times it waits for memory: lane p takes
+// part p's (m, l), and the first parts' rows are asked for at the same time.
+// It starts while k_attend_packed's last CTAs run and waits for them here.
 template <int DT>
 __global__ void __launch_bounds__(256) k_packed_combine(const PackedArgs a) {
   const PackedUnit u = a.units[blockIdx.x];
   const int lane = int(threadIdx.x) & 31;
   const int row = int(blockIdx.y) * 8 + (int(threadIdx.x) >> 5);
-  if (row >= u.rows) return;
   const int G = a.G, r = u.row0 + row, tok = r / G, h = u.kvh * G + r - tok * G;
   const int64_t q = int64_t(u.q_start) + tok;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
-  float M = -INFINITY;
-  for (int p = 0; p < u.parts; ++p) M = fmaxf(M, ml[int64_t(u.part_row) + int64_t(p) * u.rows + row].x);
-  float zh = -INFINITY;
-  if (a.hist_o) zh = __ldg(a.hist_lse + int64_t(h) * a.hist_lse_head + q) * 1.4426950408889634f;
-  M = fmaxf(M, zh);
-  const float nm = M == -INFINITY ? 0.0f : M;
   const bool live = 4 * lane < a.D;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (row >= u.rows) return;
+  float M = -INFINITY, L = 0.0f;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float L = 0.0f;
-  if (a.hist_o) {
-    const float w = exp2f(zh - nm);
-    L = w;
-    if (live && w != 0.0f) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(a.hist_o + (q * a.H + h) * a.D) + lane);
-      acc = make_float4(w * x.x, w * x.y, w * x.z, w * x.w);
+  if (a.hist_o) {  // a first part of sum 1
+    const float4 x = live ? __ldg(reinterpret_cast<const float4*>(a.hist_o + (q * a.H + h) * a.D) + lane) : acc;
+    M = __ldg(a.hist_lse + int64_t(h) * a.hist_lse_head + q) * 1.4426950408889634f;
+    if (M != -INFINITY) {  // (a NaN stays in the sum)
+      L = M == M ? 1.0f : M;
+      acc = x;
     }
   }
-  for (int p = 0; p < u.parts; ++p) {
-    const int64_t pr = int64_t(u.part_row) + int64_t(p) * u.rows + row;
-    const float2 v = ml[pr];
-    const float w = exp2f(v.x - nm);
-    L = fmaf(w, v.y, L);
-    if (live && (w != 0.0f || w != w)) {
-      const float4 o = reinterpret_cast<const float4*>(a.part_o + pr * a.D)[lane];
-      acc.x = fmaf(w, o.x, acc.x);
-      acc.y = fmaf(w, o.y, acc.y);
-      acc.z = fmaf(w, o.z, acc.z);
-      acc.w = fmaf(w, o.w, acc.w);
+  constexpr int kBatch = 8;
+  for (int p0 = 0; p0 < u.parts; p0 += 32) {
+    const int cnt = min(32, u.parts - p0);
+    const int64_t first = int64_t(u.part_row) + int64_t(p0) * u.rows + row;
+    float2 v = make_float2(-INFINITY, 0.0f);
+    if (lane < cnt) v = reinterpret_cast<const float2*>(a.part_ml)[first + int64_t(lane) * u.rows];
+    float w = 0.0f;  // this lane's part's weight
+    for (int b = 0; b < cnt; b += kBatch) {
+      float4 o[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        if (live && b + k < cnt)
+          o[k] = reinterpret_cast<const float4*>(a.part_o + (first + int64_t(b + k) * u.rows) * a.D)[lane];
+      if (b == 0) {
+        float top = v.x;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        const float to = fmaxf(M, top), nm = to == -INFINITY ? 0.0f : to;
+        const float keep = M == -INFINITY ? 1.0f : exp2f(M - nm);  // (nothing yet: L and acc are 0)
+        w = exp2f(v.x - nm);
+        float l = w * v.y;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, d);
+        L = fmaf(L, keep, l);
+        acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
+        M = to;
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float wk = __shfl_sync(0xFFFFFFFFu, w, b + k);
+        if (live && b + k < cnt && (wk != 0.0f || wk != wk)) {
+          acc.x = fmaf(wk, o[k].x, acc.x);
+          acc.y = fmaf(wk, o[k].y, acc.y);
+          acc.z = fmaf(wk, o[k].z, acc.z);
+          acc.w = fmaf(wk, o[k].w, acc.w);
+        }
+      }
     }
   }
   const bool empty = L == 0.0f;
@@ -882,8 +918,15 @@ cudaError_t launch_shape(const Maps& m, const PackedArgs& a, cudaStream_t s) {
   k_attend_packed<DT, DP><<<unsigned(a.n_ctas), kThreads, Shape<DP>::kSmem, s>>>(m.q, m.k, m.v, m.h, a);
   e = cudaGetLastError();
   if (e != cudaSuccess || a.n_units == 0) return e;
-  k_packed_combine<DT><<<dim3(unsigned(a.n_units), unsigned((a.max_unit_rows + 7) / 8)), 256, 0, s>>>(a);
-  return cudaGetLastError();
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(a.n_units), unsigned((a.max_unit_rows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cfg.attrs = &early, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_packed_combine<DT>, a);
 }
 
 }  // namespace

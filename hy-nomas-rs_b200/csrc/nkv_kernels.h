@@ -353,6 +353,7 @@ struct PackedUnit {
 struct PackedArgs {
   const PackedItem* items;      // by CTA
   const int32_t* cta_begin;     // [n_ctas + 1]
+  const PackedItem* first;      // [n_ctas] each CTA's first item once more
   const PackedUnit* units;
   int32_t n_ctas, n_units, max_unit_rows;
   int32_t H, G, D;
