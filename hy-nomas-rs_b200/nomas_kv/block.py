@@ -117,8 +117,14 @@ def _enter(index, stream, tensors):
 
 
 def _extent(t) -> int:
-    """Elements from the first to one past the last of a non-empty tensor."""
-    return 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    """Bytes from the first element to the end of the last of a non-empty tensor."""
+    es = t.element_size()
+    if t.is_contiguous():
+        return t.numel() * es
+    n = 1
+    for size, stride in zip(t.shape, t.stride()):
+        n += (size - 1) * stride
+    return n * es
 
 
 def _overlap(a, b) -> bool:
@@ -127,14 +133,15 @@ def _overlap(a, b) -> bool:
     if a is None or b is None or a.numel() == 0 or b.numel() == 0:
         return False
     pa, pb = a.data_ptr(), b.data_ptr()
-    if pa + _extent(a) * a.element_size() <= pb or pb + _extent(b) * b.element_size() <= pa:
+    if (pa + _extent(a) <= pb) if pa <= pb else (pb + _extent(b) <= pa):
         return False
-    pitch = a.stride(0) * a.element_size()
-    if pitch == b.stride(0) * b.element_size() and a.shape[0] > 1 and b.shape[0] > 1:
-        ea, eb = _extent(a[0]) * a.element_size(), _extent(b[0]) * b.element_size()
-        if ea <= pitch and eb <= pitch:
-            d = (pb - pa) % pitch
-            return d < ea or d + eb > pitch
+    if a.dim() and b.dim():
+        pitch = a.stride(0) * a.element_size()
+        if pitch == b.stride(0) * b.element_size() and a.shape[0] > 1 and b.shape[0] > 1:
+            ea, eb = _extent(a[0]), _extent(b[0])
+            if ea <= pitch and eb <= pitch:
+                d = (pb - pa) % pitch
+                return d < ea or d + eb > pitch
     return True
 
 
@@ -144,6 +151,8 @@ def _same(a, b) -> bool:
 
 def _dense_order(t) -> bool:
     """No two elements of t share memory (the strides nest)."""
+    if t.is_contiguous():
+        return True
     need = 1
     for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda p: p[1]):
         if s < need:
@@ -172,7 +181,7 @@ def _check_out(out, like, ins, name: str, alias=(), others=()):
     if not _dense_order(out):
         raise GeometryError(f"elements of {name} overlap")
     for t in ins:
-        if _overlap(out, t) and not (any(t is a for a in alias) and _same(out, t)):
+        if t is not None and not (_same(out, t) and any(t is x for x in alias)) and _overlap(out, t):
             raise ArgumentError(f"{name} overlaps an input")
     if any(_overlap(out, t) for t in others):
         raise ArgumentError(f"{name} overlaps another output")
