@@ -19,7 +19,7 @@
 // 5,120 columns, too few loads in flight for HBM if they went to registers as
 // well: rows arrive by cp.async, several ahead, each thread waiting for its own
 // bytes only.  Measured: 6,496 rows of 5,120 bf16 columns with norms on both
-// sides and five modulation groups (266 MB): 54 us, 4.9 TB/s, where a plain
+// sides and five modulation groups (266 MB): 53 us, 5.1 TB/s, where a plain
 // copy of as many bytes takes 47.  One row: 5 us, a launch.
 #include <algorithm>
 
@@ -191,11 +191,13 @@ __device__ __forceinline__ void products8(const ResidualNormParams& a, int g, in
 // bytes of its chunks of the kAhead rows on their way.
 //
 // 96 registers a thread, so that two CTAs of 320 threads share an SM (at 100
-// one does: 108 us for the 266 MB above, against 87 then).  The instructions
+// only one does).  The instructions
 // count next: addresses that advance row by row, and x unpacked only when the
 // branch's norm is known, took 583 instructions per row and warp to 427 and
-// 61 us to 54 (8,192 columns: 94 to 75).
-template <int DT, int kAhead>
+// 61 us to 54 (8,192 columns: 94 to 75).  Two rows on their way are enough (53
+// us; without modulation groups 49, with three or four rows 52).
+constexpr int kAhead = 2;
+template <int DT>
 __global__ void __maxnreg__(96) k_residual_norm_vec(const ResidualNormParams a) {
   extern __shared__ uint4 ring[];
   __shared__ float4 part[16];
@@ -403,34 +405,30 @@ __global__ void __launch_bounds__(kMaxThreads) k_residual_norm_any(const Residua
   put_row<DT>(a.y_out, int64_t(t) * a.y_stride, n, threads, h);
 }
 
-template <int DT, int kAhead>
-cudaError_t launch_vec(ResidualNormParams a, size_t row, cudaStream_t s) {
+template <int DT>
+cudaError_t launch_vec(ResidualNormParams a, cudaStream_t s) {
   const int64_t chunks = a.dim / 8;
   const int threads = int(((chunks + 1) / 2 + 31) / 32 * 32);
-  // as many CTAs as 96 registers a thread and the rings let an SM hold
-  const size_t smem = row * kAhead;
+  // as many CTAs as 96 registers a thread and the rings (x and branch of each
+  // row; at most 128 KB) let an SM hold
+  const size_t smem = size_t(a.dim) * 2 * dtype_size(DT) * kAhead;
   const uint64_t per_sm = std::max<uint64_t>(1, std::min<uint64_t>({640u / uint64_t(threads), 220 * 1024 / (smem + 1280), 12}));
   a.rows_per_cta = (a.tokens + per_sm * 148 - 1) / (per_sm * 148);
   const unsigned grid = unsigned((a.tokens + a.rows_per_cta - 1) / a.rows_per_cta);
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(k_residual_norm_vec<DT, kAhead>,
+    const cudaError_t e = cudaFuncSetAttribute(k_residual_norm_vec<DT>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
     if (e != cudaSuccess) return e;
   }
-  k_residual_norm_vec<DT, kAhead><<<grid, threads, smem, s>>>(a);
+  k_residual_norm_vec<DT><<<grid, threads, smem, s>>>(a);
   return cudaGetLastError();
-}
-
-// x and branch of a row in the ring: four rows where two CTAs' rings then fit
-// an SM, else two (of at most 64 KB).
-template <int DT>
-cudaError_t launch_vec(const ResidualNormParams& a, cudaStream_t s) {
-  const size_t row = size_t(a.dim) * 2 * dtype_size(DT);
-  return row * 4 <= 100 * 1024 ? launch_vec<DT, 4>(a, row, s) : launch_vec<DT, 2>(a, row, s);
 }
 
 template <int DT>
 cudaError_t launch_any(const ResidualNormParams& a, cudaStream_t s) {
+  // values per thread: 8 up to 2,048 columns (20,000 rows of 130: 21 us, with 16
+  // 33; of 1,155 the same); four rows of one warp each in a CTA (of 255: 23 us
+  // against 25 alone)
   const int per = a.dim <= 2048 ? 8 : 16;
   const int threads = a.dim <= 16384 ? int((a.dim + 32 * per - 1) / (32 * per) * 32) : 1024;
   const dim3 block(threads, threads == 32 ? 4 : 1);

@@ -38,6 +38,19 @@
 //
 // Every wait on an mbarrier gives up after 1 s, sets bit 0 of the plan's
 // status word, frees the TMEM and returns.
+//
+// Measured, and what bounds it (copy 6.5 TB/s, matrix product 1,679 TFLOP/s):
+// - 6,496 frame-causal queries, 24 heads of 128, history merged (319 GFLOP):
+//   300 to 350 us by the GPU's power limit (clock down to 1,650 MHz), 0.9 to
+//   1.05 PFLOP/s; tensor pipe 59 %, issue 52 %: the softmax warps' chain of
+//   latencies per step (about 1,450 cycles for both halves, 1,280 of them tensor
+//   time at head_dim 128: S at N = 64 takes 48 cycles per MMA, bound by shared
+//   memory, where N = 128 would need 512 more TMEM columns).
+// - 16,383 causal queries, 16 heads of 64 (550 GFLOP): 800 us, 0.69 PFLOP/s, the
+//   exponentials and that chain.
+// - one token over 29,056 keys, 24 heads of 128 (357 MB): 65 us, 5.5 TB/s.
+// - chunks of 1 to 64 tokens over caches of up to 9,001 (59 MB): 26 us, of which
+//   13 the loop at memory speed, the rest start, output and merge.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -95,7 +108,8 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, i
 
 // Bounded wait as tc::bar_wait, but small: the roles' code runs from the
 // instruction cache at once, and two dozen waits with their retries unrolled
-// made it 120 KB.
+// made it 120 KB.  (A suspend-time hint on the wait: the one-token case 76 us
+// instead of 65.)
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
   if (bar_try(bar, parity)) return true;
   const uint64_t t0 = gtimer();
@@ -796,7 +810,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // L = sum_p 2^(m_p - M) l_p, lse = (M + log2 L) ln 2.  It moves a few hundred
 // kilobytes, so what counts is how many times it waits for memory: lane p takes
 // part p's (m, l), and the first parts' rows are asked for at the same time.
-// It starts while k_attend_packed's last CTAs run and waits for them here.
+// It is launched while k_attend_packed's last CTAs run and waits for them here.
+// One part after the other and launched behind: the one-token case above 69 us
+// instead of 66, the chunks 31 instead of 27.
 template <int DT>
 __global__ void __launch_bounds__(256) k_packed_combine(const PackedArgs a) {
   const PackedUnit u = a.units[blockIdx.x];
@@ -947,6 +963,8 @@ bool launch_attend_packed(PackedArgs a, int dtype, const void* k, int64_t q_toke
     return false;
   if (a.hist_o && !make_map(&m.h, a.hist_o, F32, q_tokens, a.H, a.D, int64_t(a.H) * a.D, a.D, a.G, box_tokens))
     return false;
+  // head_dim up to 64 in tiles of its own width: 4,096 queries, 24 heads of 64
+  // take 94 us, padded to 128 114; four tokens over 20,000 keys 101 and 119
   if (dtype == BF16)
     *err = a.D <= 64 ? launch_shape<BF16, 64>(m, a, s) : launch_shape<BF16, 128>(m, a, s);
   else

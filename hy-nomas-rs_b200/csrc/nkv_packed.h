@@ -118,8 +118,11 @@ inline void set_steps(PackedItem* it, int64_t G, bool causal, int64_t block) {
 
 // The schedule for `sms` SMs.  Items of two halves share each K / V tile
 // between them; with fewer of them than SMs, items of one half are weighed
-// against them.  Key ranges are split (into ranges of at least four tiles)
-// when the estimate with one to three rounds of items beats no split.
+// against them (256 queries over 512 keys, 24 heads: 14.5 us against 16.5; 640
+// over 20,000 stay in two halves: 155 against 221).  Key ranges are split (into
+// ranges of at least four tiles) when the estimate with one to three rounds of
+// items beats no split (one token over 29,056 keys, 24 heads: 65 us against
+// 305; 6,496 over 6,496 stay whole).
 inline PackedSchedule packed_schedule(const std::vector<int64_t>& q_lens, const std::vector<int64_t>& k_lens, int H,
                                       int kv_heads, bool causal, int64_t block, int sms) {
   using namespace packed_detail;
