@@ -1,10 +1,11 @@
-"""Build libnomas_kv.so (C ABI + sm_100a kernels) in-tree.
+"""Build libnomas_kv.so (C ABI + sm_100a kernels) and _block_binding.so (the
+Python extension of nomas_kv/block.py, compiled against torch) in-tree.
 
     python hy-nomas-rs_b200/build.py          # incremental
     python hy-nomas-rs_b200/build.py --clean  # from scratch
 
-Objects go to hy-nomas-rs_b200/_build/, the library to
-hy-nomas-rs_b200/nomas_kv/libnomas_kv.so (both git-ignored; the .so travels
+Objects go to hy-nomas-rs_b200/_build/, the libraries to
+hy-nomas-rs_b200/nomas_kv/ (both git-ignored; the .so travels
 with the source tree to the GPU host).  nvcc cross-compiles for sm_100a, so
 this runs on a machine without a GPU.
 """
@@ -22,6 +23,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "nomas_kv", "libnomas_kv.so")
+BINDING = os.path.join(PKG, "nomas_kv", "_block_binding.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 SOURCES = ["kernels_commit.cu", "kernels_gather.cu", "kernels_qvg.cu", "kernels_qvg_fit.cu", "kernels_project.cu",
@@ -62,12 +64,34 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _binding() -> None:
+    src, header = os.path.join(CSRC, "block_binding.cpp"), os.path.join(ROOT, "include", "nomas_kv.h")
+    if not _newer(BINDING, [src, header]):
+        return
+    import sysconfig
+
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    inc = [os.path.join(ROOT, "include"), os.path.join(base, "include"), sysconfig.get_paths()["include"],
+           os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-fPIC", "-O2", "-std=c++17", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in inc), src,
+           "-o", BINDING, f"-L{os.path.join(base, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda",
+           "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for block_binding.cpp:\n{r.stdout}\n{r.stderr}")
+
+
 def build(clean: bool = False, verbose: bool = False) -> str:
     if clean and os.path.isdir(BUILD):
         shutil.rmtree(BUILD)
     os.makedirs(BUILD, exist_ok=True)
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
+        binding = ex.submit(_binding)
         objs = list(ex.map(_compile, SOURCES))
+        binding.result()
     if _newer(LIB, objs):
         cmd = [NVCC, "-shared", "-cudart", "static", "-gencode", "arch=compute_100a,code=sm_100a", "-o", LIB, *objs,
                "-lpthread", "-ldl", "-lrt"]

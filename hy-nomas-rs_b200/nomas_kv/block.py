@@ -21,6 +21,11 @@ import torch
 
 from . import ArgumentError, CudaError, GeometryError, InvalidConfigError, _abi, _check, lib
 
+try:
+    from . import _block_binding
+except ImportError as e:
+    raise ImportError(f"{e}; build it with: python hy-nomas-rs_b200/build.py") from e
+
 __all__ = ["RotaryAxes", "rope_tables", "rotary", "residual_norm", "AttendPlan", "attend_packed"]
 
 _CODES = {torch.float32: _abi.NKV_F32, torch.bfloat16: _abi.NKV_BF16, torch.float16: _abi.NKV_F16}
@@ -29,13 +34,18 @@ _NORMS = {None: _abi.NKV_NORM_NONE, "none": _abi.NKV_NORM_NONE, "rms": _abi.NKV_
           "layer": _abi.NKV_NORM_LAYER}
 
 
-# A call of a few microseconds of GPU work is bound by what happens here, so
-# the argument structs are packed in one go (native layout, as the header's)
-# and the checks read each attribute once.
+# A call of a few microseconds of GPU work is bound by what happens here.  The
+# plain calls (own outputs, torch's current device and stream) go through the
+# compiled binding, which returns None for whatever it does not take: the code
+# below then serves the call or says what is wrong with it.  It packs the
+# argument structs in one go (native layout, as the header's).
+_block_binding.bind(*(C.cast(getattr(lib(), f), C.c_void_p).value
+                      for f in ("nkv_rope_tables", "nkv_rotary", "nkv_residual_norm", "nkv_attend_packed")))
 _AXES = struct.Struct("i4iid")
 _ROTARY = struct.Struct("32sPiiQiif" + "PPqqqqPi0P" * 2)
 _NORM = struct.Struct("QqiiiiifPPPPqqqqPPPPPPi0P")
 _ATTEND = struct.Struct("iiQQPPPqqqqqqfPPPPPQ")
+_PLAN = struct.Struct("QiiiiQQQ")
 for _s, _t in ((_AXES, _abi.nkv_rope_axes), (_ROTARY, _abi.nkv_rotary_args), (_NORM, _abi.nkv_residual_norm_args),
                (_ATTEND, _abi.nkv_attend_args)):
     assert _s.size == C.sizeof(_t), _t.__name__
@@ -233,6 +243,10 @@ def rope_tables(positions, axes: RotaryAxes, cos=None, sin=None, stream=None):
     """The (cos, sin) f32 tables (tokens, axes.pairs) of nkv_rope_tables: what
     kv_project takes as `rope` (64 pairs).  positions: (tokens, n_axes) int32,
     int64 or f32."""
+    if cos is None and sin is None and stream is None:
+        done = _block_binding.rope_tables(axes._packed, positions)
+        if done is not None:
+            return done
     index = _device_of(positions, cos, sin)
     code = _positions(positions, axes, None)
     shape = (positions.shape[0], axes.pairs)
@@ -264,6 +278,10 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
     dimension dense, so q and k may be views of one fused projection.  q_out /
     k_out may be q / k themselves (in place, where k is not q).  Returns q_out, or (q_out,
     k_out) when k is given."""
+    if q_out is None and k_out is None and stream is None:
+        done = _block_binding.rotary(axes._packed, positions, q, k, norm, q_weight, k_weight, eps)
+        if done is not None:
+            return done
     index = _device_of(q, k, positions, q_weight, k_weight, q_out, k_out)
     code = _code(q, "q")
     if q.dim() != 3:
@@ -347,6 +365,11 @@ def residual_norm(x, branch=None, *, gate=None, post=None, post_weight=None, nor
     index is out of range gets NaN).  Without a branch h is x; with norm None
     y is None.  h_out / y_out may be x or branch.  Returns (h, y); y is what
     kv_project takes as x."""
+    if h_out is None and y_out is None and stream is None and post in _NORMS and norm in _NORMS:
+        done = _block_binding.residual_norm(x, branch, gate, _NORMS[post], post_weight, _NORMS[norm], weight, scale,
+                                            shift, mod_index, eps)
+        if done is not None:
+            return done
     index = _device_of(x, branch, gate, post_weight, weight, scale, shift, mod_index, h_out, y_out)
     code = _code(x, "x")
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
@@ -440,7 +463,7 @@ class AttendPlan:
 
     def __init__(self, q_lens: Sequence[int], heads: int, kv_heads: Optional[int] = None, head_dim: int = 128,
                  k_lens: Optional[Sequence[int]] = None, causal: bool = True, block: int = 1, device=None):
-        self._h = None
+        self._h = self._key = None
         q, qa = _lens(q_lens, "q_lens")
         k, ka = (q, qa) if k_lens is None else _lens(k_lens, "k_lens")
         if len(q) != len(k):
@@ -466,9 +489,12 @@ class AttendPlan:
         self.q_tokens, self.k_tokens = int(info.q_tokens), int(info.k_tokens)
         self.items, self.split_units = int(info.items), int(info.split_units)
         self.workspace_bytes = int(info.workspace_bytes)
+        self._key = _PLAN.pack(h.value, self.heads, self.kv_heads, self.head_dim, device.index, self.q_tokens,
+                               self.k_tokens, self.workspace_bytes)
 
     def close(self):
         if getattr(self, "_h", None):
+            self._key = None
             _check(lib().nkv_attend_plan_destroy(self._h))
             self._h = None
 
@@ -502,6 +528,10 @@ def attend_packed(plan: AttendPlan, q, k, v, scale: Optional[float] = None, hist
         raise ArgumentError("the plan is closed")
     H, KV, D = plan.heads, plan.kv_heads, plan.head_dim
     ho, hl = (None, None) if history is None else history
+    if out is None and lse is None and stream is None:
+        done = _block_binding.attend_packed(plan._key, q, k, v, scale, ho, hl)
+        if done is not None:
+            return done
     index = _device_of(q, k, v, ho, hl, out, lse)
     if index != plan.device.index:
         raise ArgumentError(f"the plan is for {plan.device}, the tensors are on {q.device}")

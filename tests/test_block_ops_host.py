@@ -236,3 +236,16 @@ def test_structs_match_the_header(nkv, tmp_path):
         assert int(out[name]) == C.sizeof(st), name
         for f, _ in st._fields_:
             assert int(out[f"{name}.{f}"]) == getattr(st, f).offset, f"{name}.{f}"
+
+
+def test_binding_leaves_cpu_tensors_to_the_checks(nkv):
+    import torch
+    from nomas_kv import _block_binding as fast
+    q, pos = torch.zeros((2, 1, 8)), torch.zeros((2, 1), dtype=torch.int32)
+    ax = nkv.RotaryAxes((8,))._packed
+    assert fast.rotary(ax, pos, q, None, False, None, None, 1e-6) is None
+    assert fast.rope_tables(ax, pos) is None
+    assert fast.residual_norm(q[:, 0], None, None, 0, None, 1, None, None, None, None, 1e-6) is None
+    assert fast.attend_packed(None, q, q, q, None, None, None) is None
+    with pytest.raises(TypeError):
+        fast.bind(1)
