@@ -1,11 +1,11 @@
 // block_binding.cpp — the short way from nomas_kv/block.py into the C ABI: a
 // Python extension that takes the plain calls (exact torch tensors on the
-// current device, outputs of its own, torch's current stream), checks them,
-// allocates the outputs and calls the library.  Whatever is not plain or not
+// current device, torch's current stream), checks them, allocates the outputs
+// that are not given and calls the library.  Whatever is not plain or not
 // valid returns None, and block.py's own checks run: they serve the call or
 // say what is wrong with it.  A call of a few microseconds of GPU work is bound
-// by this path: one token's rotary takes 7 us of host time here, 14 in Python (torch's own
-// addition of two rows 4.6).
+// by this path: one token's rotary takes 7 us of host time here, 14 in Python
+// (torch's own addition of two rows: 4.6).
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
@@ -16,6 +16,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
+#include <utility>
 
 #include "nomas_kv.h"
 
@@ -71,6 +73,53 @@ struct Tensors {
   }
   void* stream() const { return c10::cuda::getCurrentCUDAStream(c10::DeviceIndex(device)).stream(); }
 };
+
+int64_t bytes_of(const at::Tensor& t) {  // from the first element to the end of the last
+  if (t.numel() == 0) return 0;
+  int64_t n = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+  return n * int64_t(t.element_size());
+}
+
+// No byte in common: ranges that do not meet, or column blocks beside each
+// other in rows of one pitch.
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  const char *pa = static_cast<const char*>(a.data_ptr()), *pb = static_cast<const char*>(b.data_ptr());
+  if (pa + bytes_of(a) <= pb || pb + bytes_of(b) <= pa) return true;
+  if (a.dim() < 1 || b.dim() < 1 || a.size(0) < 2 || b.size(0) < 2) return false;
+  const int64_t pitch = a.stride(0) * int64_t(a.element_size());
+  if (pitch <= 0 || pitch != b.stride(0) * int64_t(b.element_size())) return false;
+  const int64_t ra = bytes_of(a) - (a.size(0) - 1) * pitch, rb = bytes_of(b) - (b.size(0) - 1) * pitch;
+  const int64_t d = ((pb - pa) % pitch + pitch) % pitch;
+  return ra <= pitch && rb <= pitch && d >= ra && d + rb <= pitch;
+}
+
+// A caller's output (object o) for `inputs`: shape and type as given, rows
+// dense, no element twice in memory, no byte of an input's but where it is one
+// of the `same` inputs itself.
+bool output_fits(const at::Tensor& t, PyObject* o, at::IntArrayRef shape, at::ScalarType type,
+                 std::initializer_list<std::pair<const at::Tensor*, PyObject*>> inputs, bool may_alias) {
+  if (t.sizes() != shape || t.scalar_type() != type) return false;
+  if (t.dim() && t.size(-1) > 1 && t.stride(-1) != 1) return false;
+  if (!t.is_contiguous()) {
+    int64_t need = 1;  // strides that nest, from the last dimension out
+    for (int64_t d = t.dim() - 1; d >= 0; --d) {
+      if (t.size(d) < 2) continue;
+      if (t.stride(d) < need) return false;
+      need += t.stride(d) * (t.size(d) - 1);
+    }
+  }
+  for (const auto& in : inputs)
+    if (in.first && !(may_alias && in.second == o) && !apart(t, *in.first)) return false;
+  return true;
+}
+
+PyObject* handed(PyObject* given, at::Tensor& made) {  // a new reference
+  if (given == Py_None) return THPVariable_Wrap(std::move(made));
+  Py_INCREF(given);
+  return given;
+}
 
 void* address(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
@@ -151,38 +200,49 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// rope_tables(axes, positions) -> (cos, sin)
+// rope_tables(axes, positions, cos, sin) -> (cos, sin)
 PyObject* rope_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     nkv_rope_axes axes;
-    if (n != 2 || !entries.rope_tables || !axes_of(a[0], &axes)) return nullptr;
+    if (n != 4 || !entries.rope_tables || !axes_of(a[0], &axes)) return nullptr;
     Tensors in;
-    const at::Tensor* pos = in.required(a[1]);
+    const at::Tensor *pos = in.required(a[1]), *given[2] = {in.optional(a[2]), in.optional(a[3])};
     if (!in.ok || !positions_fit(*pos, axes.n_axes)) return nullptr;
     int64_t pairs = 0;
     for (int i = 0; i < axes.n_axes && i < 4; ++i) pairs += axes.dims[i] / 2;
     const auto opt = pos->options().dtype(at::kFloat);
-    at::Tensor c = at::empty({pos->size(0), pairs}, opt), s = at::empty({pos->size(0), pairs}, opt);
+    const int64_t shape[2] = {pos->size(0), pairs};
+    at::Tensor made[2];
+    float* to[2];
+    for (int i = 0; i < 2; ++i) {
+      if (given[i] && (!given[i]->is_contiguous() ||
+                       !output_fits(*given[i], a[2 + i], shape, at::kFloat, {{pos, a[1]}, {given[1 - i], a[3 - i]}}, false)))
+        return nullptr;
+      if (!given[i]) made[i] = at::empty(shape, opt);
+      to[i] = static_cast<float*>((given[i] ? *given[i] : made[i]).data_ptr());
+    }
     void* st = in.stream();
     const void* p = pos->data_ptr();
-    float *cp = static_cast<float*>(c.data_ptr()), *sp = static_cast<float*>(s.data_ptr());
     if (!run([&] {
-          return entries.rope_tables(&axes, p, position_code(pos->scalar_type()), uint64_t(pos->size(0)), cp, sp, st);
+          return entries.rope_tables(&axes, p, position_code(pos->scalar_type()), uint64_t(pos->size(0)), to[0], to[1],
+                                     st);
         }))
       return nullptr;
-    return pair_of(THPVariable_Wrap(std::move(c)), THPVariable_Wrap(std::move(s)));
+    return pair_of(handed(a[2], made[0]), handed(a[3], made[1]));
   });
 }
 
-// rotary(axes, positions, q, k, norm, q_weight, k_weight, eps) -> q_out or (q_out, k_out)
+// rotary(axes, positions, q, k, norm, q_weight, k_weight, eps, q_out, k_out) ->
+// q_out or (q_out, k_out)
 PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     nkv_rotary_args r{};
-    if (n != 8 || !entries.rotary || !axes_of(a[0], &r.axes) || !PyBool_Check(a[4]) || !eps_of(a[7], &r.eps))
+    if (n != 10 || !entries.rotary || !axes_of(a[0], &r.axes) || !PyBool_Check(a[4]) || !eps_of(a[7], &r.eps))
       return nullptr;
     Tensors in;
     const at::Tensor *pos = in.required(a[1]), *q = in.required(a[2]), *k = in.optional(a[3]),
-                     *qw = in.optional(a[5]), *kw = in.optional(a[6]);
+                     *qw = in.optional(a[5]), *kw = in.optional(a[6]), *qo = in.optional(a[8]),
+                     *ko = in.optional(a[9]);
     if (!in.ok || q->dim() != 3 || !positions_fit(*pos, r.axes.n_axes)) return nullptr;
     const int64_t tokens = q->size(0), D = q->size(2);
     const int code = type_code(q->scalar_type());
@@ -191,14 +251,25 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
               k->stride(2) != 1))
       return nullptr;
     r.norm = a[4] == Py_True;
-    if ((!r.norm && (qw || kw)) || (!k && kw)) return nullptr;
+    if ((!r.norm && (qw || kw)) || (!k && (kw || ko))) return nullptr;
+    // (q and k one tensor: read as both, so neither may be rotated in place)
+    const bool in_place = a[2] != a[3];
+    if (qo && (!output_fits(*qo, a[8], q->sizes(), q->scalar_type(), {{pos, a[1]}, {q, a[2]}, {qw, a[5]}, {kw, a[6]}},
+                            in_place) ||
+               (k && !apart(*qo, *k)) || (ko && !apart(*qo, *ko))))
+      return nullptr;
+    if (ko && (!output_fits(*ko, a[9], k->sizes(), k->scalar_type(), {{pos, a[1]}, {k, a[3]}, {qw, a[5]}, {kw, a[6]}},
+                            in_place) ||
+               !apart(*ko, *q)))
+      return nullptr;
     for (const at::Tensor* w : {qw, kw})
       if (w && (w->dim() != 1 || w->size(0) != D || w->scalar_type() != q->scalar_type() || !w->is_contiguous()))
         return nullptr;
     at::Tensor out[2];
-    auto side = [&](const at::Tensor& t, const at::Tensor* w, at::Tensor& o) {
-      o = at::empty(t.sizes(), t.options());
-      return nkv_rotary_side{t.data_ptr(), o.data_ptr(), t.stride(0), t.stride(1), t.size(1) * D, D, address(w),
+    auto side = [&](const at::Tensor& t, const at::Tensor* w, const at::Tensor* given, at::Tensor& made) {
+      if (!given) made = at::empty(t.sizes(), t.options());
+      const at::Tensor& o = given ? *given : made;
+      return nkv_rotary_side{t.data_ptr(), o.data_ptr(), t.stride(0), t.stride(1), o.stride(0), o.stride(1), address(w),
                              int32_t(t.size(1))};
     };
     if (q->size(1) > 65535 || (k && k->size(1) > 65535)) return nullptr;
@@ -207,27 +278,28 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     r.dtype = code;
     r.tokens = uint64_t(tokens);
     r.head_dim = int32_t(D);
-    r.q = side(*q, qw, out[0]);
-    if (k) r.k = side(*k, kw, out[1]);
+    r.q = side(*q, qw, qo, out[0]);
+    if (k) r.k = side(*k, kw, ko, out[1]);
     void* st = in.stream();
     if (!run([&] { return entries.rotary(&r, st); })) return nullptr;
-    PyObject* qo = THPVariable_Wrap(std::move(out[0]));
-    return k ? pair_of(qo, THPVariable_Wrap(std::move(out[1]))) : qo;
+    PyObject* first = handed(a[8], out[0]);
+    return k ? pair_of(first, handed(a[9], out[1])) : first;
   });
 }
 
 // residual_norm(x, branch, gate, post, post_weight, norm, weight, scale, shift,
-// mod_index, eps) -> (h, y); post and norm as nkv_norm_kind
+// mod_index, eps, h_out, y_out) -> (h, y); post and norm as nkv_norm_kind
 PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     nkv_residual_norm_args r{};
-    if (n != 11 || !entries.residual_norm || !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[5]) ||
+    if (n != 13 || !entries.residual_norm || !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[5]) ||
         !eps_of(a[10], &r.eps))
       return nullptr;
     r.post = int32_t(PyLong_AsLong(a[3]));
     r.norm = int32_t(PyLong_AsLong(a[5]));
     Tensors in;
-    const at::Tensor *x = in.required(a[0]), *branch = in.optional(a[1]), *index = in.optional(a[9]);
+    const at::Tensor *x = in.required(a[0]), *branch = in.optional(a[1]), *index = in.optional(a[9]),
+                     *ho = in.optional(a[11]), *yo = in.optional(a[12]);
     const at::Tensor* mods[3] = {in.optional(a[2]), in.optional(a[7]), in.optional(a[8])};  // gate, scale, shift
     const at::Tensor* weights[2] = {in.optional(a[4]), in.optional(a[6])};                  // post's, norm's
     if (!in.ok || x->dim() != 2) return nullptr;
@@ -238,8 +310,15 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (code < 0 || dim < 1 || dim > 32768 || !dense_rows(*x)) return nullptr;
     if (branch && (branch->sizes() != x->sizes() || branch->scalar_type() != type || !dense_rows(*branch)))
       return nullptr;
-    if (!branch && (r.post || mods[0] || weights[0] || !r.norm)) return nullptr;
-    if (!r.norm && (weights[1] || mods[1] || mods[2])) return nullptr;
+    if (!branch && (r.post || mods[0] || weights[0] || !r.norm || ho)) return nullptr;
+    if (!r.norm && (weights[1] || mods[1] || mods[2] || yo)) return nullptr;
+    auto fits = [&](const at::Tensor& t, PyObject* o) {
+      if (!output_fits(t, o, x->sizes(), type, {{x, a[0]}, {branch, a[1]}}, true)) return false;
+      for (const at::Tensor* v : {mods[0], mods[1], mods[2], weights[0], weights[1], index})
+        if (v && !apart(t, *v)) return false;
+      return true;
+    };
+    if ((ho && !fits(*ho, a[11])) || (yo && !fits(*yo, a[12])) || (ho && yo && !apart(*ho, *yo))) return nullptr;
     r.weight_dtype = r.mod_dtype = code;
     bool seen = false;
     for (const at::Tensor* w : weights) {
@@ -268,15 +347,16 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
               : groups > 1)
       return nullptr;
     at::Tensor h, y;
-    if (branch) h = at::empty(x->sizes(), x->options());
-    if (r.norm) y = at::empty(x->sizes(), x->options());
+    if (branch && !ho) h = at::empty(x->sizes(), x->options());
+    if (r.norm && !yo) y = at::empty(x->sizes(), x->options());
+    const at::Tensor &hr = ho ? *ho : h, &yr = yo ? *yo : y;
     r.tokens = uint64_t(tokens);
     r.dim = dim;
     r.dtype = code;
     r.x = x->data_ptr(), r.x_stride = x->stride(0);
     if (branch) r.branch = branch->data_ptr(), r.branch_stride = branch->stride(0);
-    if (branch) r.h_out = h.data_ptr(), r.h_stride = dim;
-    if (r.norm) r.y_out = y.data_ptr(), r.y_stride = dim;
+    if (branch) r.h_out = hr.data_ptr(), r.h_stride = hr.stride(0);
+    if (r.norm) r.y_out = yr.data_ptr(), r.y_stride = yr.stride(0);
     r.post_weight = address(weights[0]), r.weight = address(weights[1]);
     r.gate = address(mods[0]), r.scale = address(mods[1]), r.shift = address(mods[2]);
     r.mod_index = static_cast<const int32_t*>(address(index));
@@ -284,10 +364,10 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* st = in.stream();
     if (!run([&] { return entries.residual_norm(&r, st); })) return nullptr;
     PyObject* first = a[0];
-    if (branch) first = THPVariable_Wrap(std::move(h));
+    if (branch) first = handed(a[11], h);
     else Py_INCREF(first);
     PyObject* second = Py_None;
-    if (r.norm) second = THPVariable_Wrap(std::move(y));
+    if (r.norm) second = handed(a[12], y);
     else Py_INCREF(second);
     return pair_of(first, second);
   });
@@ -300,11 +380,11 @@ struct PlanKey {
   uint64_t q_tokens, k_tokens, workspace;
 };
 
-// attend_packed(key, q, k, v, scale or None, history's o, its lse) -> (out, lse)
+// attend_packed(key, q, k, v, scale or None, history's o, its lse, out, lse) -> (out, lse)
 PyObject* attend_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     PlanKey plan;
-    if (n != 7 || !entries.attend_packed || !PyBytes_CheckExact(a[0]) ||
+    if (n != 9 || !entries.attend_packed || !PyBytes_CheckExact(a[0]) ||
         PyBytes_GET_SIZE(a[0]) != Py_ssize_t(sizeof(plan)))
       return nullptr;
     std::memcpy(&plan, PyBytes_AS_STRING(a[0]), sizeof(plan));
@@ -312,7 +392,7 @@ PyObject* attend_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[4] != Py_None && (!number(a[4], &scale) || !(scale > 0.0 && scale <= 3.4e38))) return nullptr;
     Tensors in;
     const at::Tensor *q = in.required(a[1]), *k = in.required(a[2]), *v = in.required(a[3]), *ho = in.optional(a[5]),
-                     *hl = in.optional(a[6]);
+                     *hl = in.optional(a[6]), *out = in.optional(a[7]), *lse = in.optional(a[8]);
     const int64_t H = plan.heads, KV = plan.kv_heads, D = plan.head_dim, rows = int64_t(plan.q_tokens);
     if (!in.ok || in.device != plan.device || (ho == nullptr) != (hl == nullptr)) return nullptr;
     const at::ScalarType type = q->scalar_type();
@@ -336,16 +416,26 @@ PyObject* attend_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
                hl->size(0) != H || hl->size(1) != rows || ho->scalar_type() != at::kFloat ||
                hl->scalar_type() != at::kFloat || !ho->is_contiguous() || !hl->is_contiguous()))
       return nullptr;
-    at::Tensor out = at::empty({rows, H, D}, q->options());
-    at::Tensor lse = at::empty({H, rows}, q->options().dtype(at::kFloat)), ws;
+    const int64_t shape[3] = {rows, H, D}, lse_shape[2] = {H, rows};
+    const at::ScalarType out_type = out && out->scalar_type() == at::kFloat ? at::kFloat : type;
+    if (out && (!out->is_contiguous() || (lse && !apart(*out, *lse)) ||
+                !output_fits(*out, a[7], shape, out_type, {{q, a[1]}, {k, a[2]}, {v, a[3]}, {ho, a[5]}, {hl, a[6]}}, false)))
+      return nullptr;
+    if (lse && (!lse->is_contiguous() || !output_fits(*lse, a[8], lse_shape, at::kFloat,
+                                                      {{q, a[1]}, {k, a[2]}, {v, a[3]}, {ho, a[5]}, {hl, a[6]}}, false)))
+      return nullptr;
+    at::Tensor made, made_lse, ws;
+    if (!out) made = at::empty(shape, q->options());
+    if (!lse) made_lse = at::empty(lse_shape, q->options().dtype(at::kFloat));
     if (plan.workspace) ws = at::empty({int64_t(plan.workspace)}, q->options().dtype(at::kByte));
-    r.dtype = r.out_dtype = type_code(type);
+    r.dtype = type_code(type);
+    r.out_dtype = type_code(out_type);
     r.q_rows = uint64_t(rows);
     r.k_rows = uint64_t(std::min(k->size(0), v->size(0)));
     r.q = q->data_ptr(), r.k = k->data_ptr(), r.v = v->data_ptr();
     r.scale = float(scale);
-    r.out = out.data_ptr();
-    r.lse = static_cast<float*>(lse.data_ptr());
+    r.out = (out ? *out : made).data_ptr();
+    r.lse = static_cast<float*>((lse ? *lse : made_lse).data_ptr());
     r.hist_out = static_cast<const float*>(address(ho));
     r.hist_lse = static_cast<const float*>(address(hl));
     if (plan.workspace) r.workspace = ws.data_ptr();
@@ -353,7 +443,7 @@ PyObject* attend_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* st = in.stream();
     if (!run([&] { return entries.attend_packed(reinterpret_cast<const nkv_attend_plan*>(plan.plan), &r, st); }))
       return nullptr;
-    return pair_of(THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
+    return pair_of(handed(a[7], made), handed(a[8], made_lse));
   });
 }
 

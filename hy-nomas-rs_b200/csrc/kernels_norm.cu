@@ -347,9 +347,10 @@ __device__ __forceinline__ void put_row(void* p, int64_t base, int n, int thread
 // can, 6,496 rows of 5,120 columns take 152 us here, 52 there; of 128 columns 9
 // and 8): blockDim.x threads per row, each holding the E
 // values tid, tid + blockDim.x, ...; one row per CTA, or one per warp when 32
-// threads suffice.
+// threads suffice.  Up to 2,048 columns at 40 registers, for more rows at once
+// (6,000 rows of 2,047: 53 us; at 48 58, at 32 54).
 template <int DT, int E, int kMaxThreads>
-__global__ void __launch_bounds__(kMaxThreads) k_residual_norm_any(const ResidualNormParams a) {
+__global__ void __launch_bounds__(kMaxThreads, kMaxThreads == 256 ? 6 : 1) k_residual_norm_any(const ResidualNormParams a) {
   __shared__ float4 part[16];
   int slot = 0;
   const int tid = int(threadIdx.x), threads = int(blockDim.x), dim = int(a.dim);

@@ -35,7 +35,7 @@ _NORMS = {None: _abi.NKV_NORM_NONE, "none": _abi.NKV_NORM_NONE, "rms": _abi.NKV_
 
 
 # A call of a few microseconds of GPU work is bound by what happens here.  The
-# plain calls (own outputs, torch's current device and stream) go through the
+# plain calls (torch's current device and stream) go through the
 # compiled binding, which returns None for whatever it does not take: the code
 # below then serves the call or says what is wrong with it.  It packs the
 # argument structs in one go (native layout, as the header's).
@@ -243,8 +243,8 @@ def rope_tables(positions, axes: RotaryAxes, cos=None, sin=None, stream=None):
     """The (cos, sin) f32 tables (tokens, axes.pairs) of nkv_rope_tables: what
     kv_project takes as `rope` (64 pairs).  positions: (tokens, n_axes) int32,
     int64 or f32."""
-    if cos is None and sin is None and stream is None:
-        done = _block_binding.rope_tables(axes._packed, positions)
+    if stream is None:
+        done = _block_binding.rope_tables(axes._packed, positions, cos, sin)
         if done is not None:
             return done
     index = _device_of(positions, cos, sin)
@@ -278,8 +278,8 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
     dimension dense, so q and k may be views of one fused projection.  q_out /
     k_out may be q / k themselves (in place, where k is not q).  Returns q_out, or (q_out,
     k_out) when k is given."""
-    if q_out is None and k_out is None and stream is None:
-        done = _block_binding.rotary(axes._packed, positions, q, k, norm, q_weight, k_weight, eps)
+    if stream is None:
+        done = _block_binding.rotary(axes._packed, positions, q, k, norm, q_weight, k_weight, eps, q_out, k_out)
         if done is not None:
             return done
     index = _device_of(q, k, positions, q_weight, k_weight, q_out, k_out)
@@ -365,9 +365,9 @@ def residual_norm(x, branch=None, *, gate=None, post=None, post_weight=None, nor
     index is out of range gets NaN).  Without a branch h is x; with norm None
     y is None.  h_out / y_out may be x or branch.  Returns (h, y); y is what
     kv_project takes as x."""
-    if h_out is None and y_out is None and stream is None and post in _NORMS and norm in _NORMS:
+    if stream is None and post in _NORMS and norm in _NORMS:
         done = _block_binding.residual_norm(x, branch, gate, _NORMS[post], post_weight, _NORMS[norm], weight, scale,
-                                            shift, mod_index, eps)
+                                            shift, mod_index, eps, h_out, y_out)
         if done is not None:
             return done
     index = _device_of(x, branch, gate, post_weight, weight, scale, shift, mod_index, h_out, y_out)
@@ -528,8 +528,8 @@ def attend_packed(plan: AttendPlan, q, k, v, scale: Optional[float] = None, hist
         raise ArgumentError("the plan is closed")
     H, KV, D = plan.heads, plan.kv_heads, plan.head_dim
     ho, hl = (None, None) if history is None else history
-    if out is None and lse is None and stream is None:
-        done = _block_binding.attend_packed(plan._key, q, k, v, scale, ho, hl)
+    if stream is None:
+        done = _block_binding.attend_packed(plan._key, q, k, v, scale, ho, hl, out, lse)
         if done is not None:
             return done
     index = _device_of(q, k, v, ho, hl, out, lse)

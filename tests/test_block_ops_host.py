@@ -243,9 +243,9 @@ def test_binding_leaves_cpu_tensors_to_the_checks(nkv):
     from nomas_kv import _block_binding as fast
     q, pos = torch.zeros((2, 1, 8)), torch.zeros((2, 1), dtype=torch.int32)
     ax = nkv.RotaryAxes((8,))._packed
-    assert fast.rotary(ax, pos, q, None, False, None, None, 1e-6) is None
-    assert fast.rope_tables(ax, pos) is None
-    assert fast.residual_norm(q[:, 0], None, None, 0, None, 1, None, None, None, None, 1e-6) is None
-    assert fast.attend_packed(None, q, q, q, None, None, None) is None
+    assert fast.rotary(ax, pos, q, None, False, None, None, 1e-6, None, None) is None
+    assert fast.rope_tables(ax, pos, None, None) is None
+    assert fast.residual_norm(q[:, 0], None, None, 0, None, 1, None, None, None, None, 1e-6, None, None) is None
+    assert fast.attend_packed(None, q, q, q, None, None, None, None, None) is None
     with pytest.raises(TypeError):
         fast.bind(1)

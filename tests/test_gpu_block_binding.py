@@ -115,7 +115,7 @@ def test_other_calls_are_left_to_the_other_path(nkv):
     q = torch.randn((4, 2, 64), device="cuda")
     pos, ax = torch.zeros((4, 2), dtype=torch.int32, device="cuda"), nkv.RotaryAxes((32, 32))._packed
     w, e = torch.ones(64, device="cuda"), 1e-6
-    assert fast.rotary(ax, pos, q, None, True, w, None, e) is not None
+    assert fast.rotary(ax, pos, q, None, True, w, None, e, None, None) is not None
     leaf = q.clone().requires_grad_()
     for args in ((ax, pos, leaf, None, False, None, None, e), (ax, pos.cpu(), q, None, False, None, None, e),
                  (ax, pos, q.cpu(), None, False, None, None, e), (ax, pos[:3], q, None, False, None, None, e),
@@ -127,14 +127,15 @@ def test_other_calls_are_left_to_the_other_path(nkv):
                  (ax[:-1], pos, q, None, False, None, None, e), (ax, pos, None, None, False, None, None, e),
                  (ax, pos, "q", None, False, None, None, e), (ax, pos, q), (),
                  (nkv.RotaryAxes((64, 64))._packed, pos, q, None, False, None, None, e)):
+        assert fast.rotary(*args, None, None) is None
         assert fast.rotary(*args) is None
     with torch.no_grad():
-        assert fast.rotary(ax, pos, leaf, None, False, None, None, e) is not None
-    assert fast.rope_tables(ax, pos.double()) is None and fast.rope_tables(ax, pos[:, :1]) is None
+        assert fast.rotary(ax, pos, leaf, None, False, None, None, e, None, None) is not None
+    assert fast.rope_tables(ax, pos.double(), None, None) is None and fast.rope_tables(ax, pos[:, :1], None, None) is None
     x, m = torch.randn((4, 32), device="cuda"), torch.randn((2, 32), device="cuda")
     i = torch.zeros(4, dtype=torch.int32, device="cuda")
     full = dict(x=x, branch=x.clone(), gate=m, post=1, post_weight=m[0], norm=1, weight=m[0], scale=m, shift=m, mod_index=i,
-                eps=e)
+                eps=e, h_out=None, y_out=None)
     assert fast.residual_norm(*full.values()) is not None
     for kw in (dict(branch=None), dict(branch=x[:3]), dict(gate=m[:, :31]), dict(gate=m[:1]), dict(mod_index=None),
                dict(mod_index=i.long()), dict(norm=0), dict(post=7), dict(norm=-1), dict(weight=m[0].half()),
@@ -145,18 +146,100 @@ def test_other_calls_are_left_to_the_other_path(nkv):
     b = torch.randn((4, 2, 64), device="cuda").bfloat16()
     plan = nkv.AttendPlan([4], 2, head_dim=64)
     key = plan._key
-    assert fast.attend_packed(key, b, b, b, None, None, None) is not None
+    assert fast.attend_packed(key, b, b, b, None, None, None, None, None) is not None
     big = torch.randn((5, 2, 64), device="cuda").bfloat16()
     ho, hl = torch.zeros((4, 2, 64), device="cuda"), torch.zeros((2, 4), device="cuda")
-    assert fast.attend_packed(key, b, big, big, None, ho, hl) is not None
+    assert fast.attend_packed(key, b, big, big, None, ho, hl, None, None) is not None
     off = torch.empty(4 * 2 * 64 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4, 2, 64)
     for args in ((key, big, b, b, None, None, None), (key, b, b[:3], b, None, None, None), (key, b, b, b.half(), None, None, None),
                  (key, b.float(), b, b, None, None, None), (key, b, b, b, 0.0, None, None), (key, b, b, b, math.nan, None, None),
                  (key, b, b, b, 3e38, None, None), (key, b, b, b, "s", None, None), (key, b, b, b, None, ho, None),
                  (key, b, b, b, None, ho[:, :1], hl), (key, b, b, b, None, ho, hl[:, :3]), (key, b, b, off, None, None, None),
                  (key, b, b, b, None, ho.bfloat16(), hl), (None, b, b, b, None, None, None), (key, b, b, b)):
-        assert fast.attend_packed(*args) is None
+        assert fast.attend_packed(*args, None, None) is None
     plan.check()
+
+
+def test_given_outputs(nkv, both):
+    """In place, into columns of a fused buffer, into outputs of the caller's: taken, and the same values."""
+    import torch
+    T, D = 9, 64
+    buf = torch.randn((T, 5, D), device="cuda").bfloat16()
+    pos, ax = torch.randint(0, 99, (T, 2), device="cuda"), nkv.RotaryAxes((32, 32))
+    want = nkv.rotary(pos, ax, buf[:, :3], k=buf[:, 3:], norm=True)
+
+    def in_place():
+        b = buf.clone()
+        q, k = b[:, :3], b[:, 3:]
+        got = nkv.rotary(pos, ax, q, k=k, norm=True, q_out=q, k_out=k)
+        assert got[0] is q and got[1] is k
+        return b
+
+    for b in both(in_place):
+        assert torch.equal(b, torch.cat(want, dim=1))
+
+    def tables():
+        out = torch.empty((T, 32), device="cuda"), torch.empty((T, 32), device="cuda")
+        got = nkv.rope_tables(pos, ax, cos=out[0], sin=out[1])
+        assert got[0] is out[0] and got[1] is out[1]
+        return got
+    _equal(*both(tables))
+
+    x0, b0 = (torch.randn((T, 96), device="cuda").bfloat16() for _ in range(2))
+    h, y = nkv.residual_norm(x0, b0, post="rms")
+
+    def stream():
+        x, b = x0.clone(), b0.clone()
+        got = nkv.residual_norm(x, b, post="rms", h_out=x, y_out=b)
+        assert got[0] is x and got[1] is b
+        return got
+    for got in both(stream):
+        _equal(got, (h, y))
+
+    q = torch.randn((T, 2, D), device="cuda").bfloat16()
+    plan = nkv.AttendPlan([T], 2, head_dim=D)
+    for dt in (torch.bfloat16, torch.float32):
+        def attend():
+            out, lse = torch.empty((T, 2, D), dtype=dt, device="cuda"), torch.empty((2, T), device="cuda")
+            got = nkv.attend_packed(plan, q, q, q, out=out, lse=lse)
+            assert got[0] is out and got[1] is lse
+            return got
+        _equal(*both(attend))
+    plan.check()
+
+
+def test_outputs_that_do_not_fit_are_left_to_the_other_path(nkv):
+    import torch
+    from nomas_kv import _block_binding as fast
+    e, T, D = 1e-6, 4, 64
+    big = torch.randn((T + 1, 4, D), device="cuda")
+    q, pos, ax = big[:T, :2], torch.zeros((T, 2), dtype=torch.int32, device="cuda"), nkv.RotaryAxes((32, 32))._packed
+    k = big[:T, 2:]
+    one = torch.empty((T, 2, D), device="cuda")
+    for qo, ko, kk in ((q.half(), None, k), (one[:3], None, k), (one.expand(T, 2, D)[:, :1].expand(T, 2, D), None, k),
+                       (big[1:, :2], None, k), (k, None, k), (None, q, k), (one, one, k), (q, None, q), (None, q, q),
+                       (one.transpose(1, 2).contiguous().transpose(1, 2), None, k), (one, one, None),
+                       (one.cpu(), None, k), ("x", None, k), (big[:T, 1:3], None, k)):
+        assert fast.rotary(ax, pos, q, kk, False, None, None, e, qo, ko) is None
+    assert fast.rotary(ax, pos, q, k, False, None, None, e, q, k) is not None
+    t = torch.empty((T, 32), device="cuda")
+    for c, s in ((t, t), (t.half(), None), (t[:3], None), (torch.empty((32, T), device="cuda").t(), None)):
+        assert fast.rope_tables(ax, pos, c, s) is None
+    m = torch.randn((T + 1, 32), device="cuda")
+    x, b, w = m[:T], torch.randn((T, 32), device="cuda"), torch.randn(32, device="cuda")
+    for ho, yo in ((m[1:], None), (None, m[1:]), (x, x), (b, b), (x.half(), None), (w.expand(T, 32), None),
+                   (torch.empty((32, T), device="cuda").t(), None)):
+        assert fast.residual_norm(x, b, None, 0, None, 1, w, None, None, None, e, ho, yo) is None
+    assert fast.residual_norm(x, None, None, 0, None, 1, w, None, None, None, e, b, None) is None
+    assert fast.residual_norm(x, b, None, 0, None, 0, None, None, None, None, e, None, b) is None
+    a = torch.randn((T, 2, D), device="cuda").bfloat16()
+    plan = nkv.AttendPlan([T], 2, head_dim=D)
+    f = torch.empty((2, T), device="cuda")
+    for out, lse in ((a, None), (a.half(), None), (torch.empty((T + 1, 2, D), device="cuda"), None), (None, f.half()),
+                     (None, torch.empty((T, 2), device="cuda").t()), (torch.empty((2, T, D), device="cuda").transpose(0, 1), None)):
+        assert fast.attend_packed(plan._key, a, a, a, None, None, None, out, lse) is None
+    buf = torch.empty(T * 2 * D, device="cuda")
+    assert fast.attend_packed(plan._key, a, a, a, None, None, None, buf.view(T, 2, D), buf[:2 * T].view(2, T)) is None
 
 
 def test_a_captured_call(nkv):
