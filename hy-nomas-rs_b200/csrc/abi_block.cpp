@@ -164,6 +164,14 @@ struct OnDevice {
   ~OnDevice() { cudaSetDevice(prev); }
 };
 
+// Lets this thread allocate, copy and free (a plan's table, none of it work of
+// a stream's) while one of the process's streams is being captured.
+struct DuringCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  DuringCapture() { nkv::check_cuda(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode"); }
+  ~DuringCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 }  // namespace
 
 extern "C" {
@@ -308,6 +316,7 @@ int nkv_attend_plan_create(const uint64_t* q_lens, const uint64_t* k_lens, uint6
     p->n_items = int32_t(s.items.size()), p->n_units = int32_t(s.units.size());
     p->n_ctas = int32_t(s.cta_begin.size()) - 1;
     p->max_unit_rows = s.max_unit_rows;
+    DuringCapture relaxed;
     auto after = [](size_t at, size_t bytes) { return (at + bytes + 63) / 64 * 64; };
     p->ctas_off = after(p->items_off, s.items.size() * sizeof(nkv::PackedItem));
     p->first_off = after(p->ctas_off, s.cta_begin.size() * sizeof(int32_t));
@@ -340,6 +349,7 @@ int nkv_attend_plan_destroy(nkv_attend_plan* plan) {
     if (!plan) return;
     {
       OnDevice on(plan->device);
+      DuringCapture relaxed;
       if (plan->table) nkv::check_cuda(cudaFree(plan->table), "cudaFree");  // waits for work that reads the table
     }
     delete plan;

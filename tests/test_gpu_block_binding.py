@@ -242,6 +242,25 @@ def test_outputs_that_do_not_fit_are_left_to_the_other_path(nkv):
     assert fast.attend_packed(plan._key, a, a, a, None, None, None, buf.view(T, 2, D), buf[:2 * T].view(2, T)) is None
 
 
+def test_plans_made_and_dropped_during_a_capture(nkv):
+    import torch
+    q = torch.randn((20, 2, 64), device="cuda").bfloat16()
+    old, plan = nkv.AttendPlan([20], 2, head_dim=64), nkv.AttendPlan([20], 2, head_dim=64)
+    want = nkv.attend_packed(plan, q, q, q)
+    plans = []
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = nkv.attend_packed(plan, q, q, q)
+        old.close()
+        plans.append(nkv.AttendPlan([5, 15], 2, head_dim=64, causal=False))
+        got2 = nkv.attend_packed(plans[0], q, q, q)
+    g.replay()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    _equal(got2, nkv.attend_packed(plans[0], q, q, q))
+    for p in (plan, *plans):
+        p.check()
+
+
 def test_a_captured_call(nkv):
     """The binding's calls in a graph: outputs from the graph's pool, on the capturing stream."""
     import torch
