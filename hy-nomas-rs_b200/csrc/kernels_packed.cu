@@ -610,7 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int k0 = ch * 32 + 2 * j;
             const float2 x = __ffma2_rn(make_float2(sv[k0], sv[k0 + 1]), sc2, nm2);
             // a quarter of the exponentials on the FMA pipes, the others on the
-            // special-function unit, which alone would take 8 cycles each
+            // special-function unit, which alone would take 8 cycles each (16,383
+            // queries of 64: 800 us; an eighth 814, three eighths 845)
             const float2 p = j % 4 == 3 ? exp2_fma(x) : make_float2(fast_exp2(x.x), fast_exp2(x.y));
             ls[j & 3] = __fadd2_rn(ls[j & 3], p);
             w[j] = pack2<DT>(p.x, p.y);
