@@ -161,11 +161,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // 2^x on the FMA pipes: x = n + f with n the nearest integer (the low bits of x
 // + 1.5 2^23), a degree-4 polynomial of 2^f on [-1/2, 1/2] (a fit of the least
 // maximal relative error with the constant held at 1: 2.9e-6, a hundredth of
-// P's rounding), n added to the exponent.  Below 2^-125 it stays at 2^-125: 0
-// next to any row's sum.  x at most 2^7; a NaN is lost here and caught by the
-// row maximum.
+// P's rounding), n added to the exponent.  x is held at -127 from below, where
+// f = 0, the polynomial is exactly 1 and the sum of the exponents leaves the
+// bits of +0: a masked score (-inf) has P = 0.  (Held at -125 a masked key would
+// weigh 2^-125, a normal bf16 number: 8 next to a value of 3.4e38.)  Between -127
+// and -126 the result falls from 2^-126 to 0, 0 next to any row's sum.  x at most
+// 2^7; a NaN is lost here and caught by the row maximum.
 __device__ __forceinline__ float2 exp2_fma(float2 x) {
-  x = make_float2(fmaxf(x.x, -125.0f), fmaxf(x.y, -125.0f));
+  x = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
   auto both = [](float v) { return make_float2(v, v); };
   const float2 t = __fadd2_rn(x, both(12582912.0f));
   const float2 f = __ffma2_rn(__fadd2_rn(t, both(-12582912.0f)), both(-1.0f), x);
