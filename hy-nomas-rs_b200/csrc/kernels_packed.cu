@@ -26,9 +26,10 @@
 // f32 in TMEM), P written over S_h in TMEM as the A operand, the running
 // maximum moved only when a step exceeds it by more than 8 (base 2).  Scores,
 // maxima, sums and O stay in f32; P is rounded to the type of V because the
-// tensor core takes both operands in one type (an error of half a step of that
-// type per probability, the size of the output's own rounding); the sum uses
-// the unrounded values.
+// tensor core takes both operands in one type: an error of half a step of that
+// type per probability, the size of the output's own rounding, or, where that is
+// more in f16, of 2^-32 of the row's largest one (2^-32 n max|v| for n keys;
+// kRaise).  The sum uses the unrounded values.
 //
 // A key past a row's limit has P = 0, but 0 times an infinity or a NaN in its
 // V row is a NaN: the V rows that some but not all rows of an item see are
@@ -191,6 +192,16 @@ __device__ __forceinline__ float max2_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
+
+// What the running maximum m lies below a row's scores' (base 2), so that the
+// largest probabilities are 2^kRaise to 2^(kRaise + 8).  f16 has no exponents to
+// spare below: held near 1, every probability under 2^-25 of the largest became
+// 0 in P but not in the sum (131,072 keys 17.4 nats below one: 0.36 % of the
+// row's mass lost).  Raised by 2^7 (32,768 at most, of 65,504) that border is at
+// 2^-32.  l and O carry the factor as well, and m accounts for it in lse and in
+// the merge of parts.
+template <int DT>
+constexpr float kRaise = DT == F16 ? 7.0f : 0.0f;
 
 // Exponent all ones: the smallest pattern of a non-finite value without sign.
 template <int DT>
@@ -595,8 +606,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 16; j < SK; j += 16)
 #pragma unroll
           for (int c = 0; c < 8; ++c) mx[c] = max3_nan(mx[c], sv[j + c], sv[j + 8 + c]);
-        const float mt = max3_nan(max3_nan(mx[0], mx[1], mx[2]), max3_nan(mx[3], mx[4], mx[5]),
-                                  max2_nan(mx[6], mx[7])) * a.scale_log2;
+        const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), max3_nan(mx[3], mx[4], mx[5]),
+                                   max2_nan(mx[6], mx[7]));
+        const float mt = fmaf(top, a.scale_log2, -kRaise<DT>);
         const bool move = mt > m + 8.0f;
         const float mn = move ? mt : m;
         const float alpha = move ? exp2f(m - mn) : 1.0f;  // 0 on a row's first visible step

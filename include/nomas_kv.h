@@ -578,7 +578,8 @@ int nkv_attend_schedule(const uint64_t* q_lens, const uint64_t* k_lens, uint64_t
  * lse.  workspace: workspace_bytes of device memory, 16-byte aligned, used by
  * this call alone until its work is done.  Values of masked keys have no
  * effect, non-finite ones included.  The probabilities are rounded to dtype
- * before they meet V; everything else is f32. */
+ * before they meet V (half a step of it each; F16: or 2^-32 of the row's largest
+ * one, where that is more); everything else is f32. */
 typedef struct {
   int32_t dtype, out_dtype;
   uint64_t q_rows, k_rows;
