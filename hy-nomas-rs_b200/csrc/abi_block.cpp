@@ -378,6 +378,16 @@ int nkv_attend_plan_status(const nkv_attend_plan* plan, uint32_t* status) {
   });
 }
 
+int nkv_attend_plan_set_status(nkv_attend_plan* plan, uint32_t status) {
+  return nkv::guarded_call([&] {
+    need(plan, "plan");
+    OnDevice on(plan->device);
+    nkv::check_cuda(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+    nkv::check_cuda(cudaMemcpy(plan->table, &status, sizeof(uint32_t), cudaMemcpyHostToDevice), "cudaMemcpy");
+    nkv::check_cuda(cudaStreamSynchronize(nullptr), "cudaStreamSynchronize");  // as in nkv_attend_plan_create
+  });
+}
+
 int nkv_attend_packed(const nkv_attend_plan* plan, const nkv_attend_args* a, void* stream) {
   return nkv::guarded_call([&] {
     need(plan, "plan");

@@ -37,8 +37,10 @@
 // rows that none sees zeroed), and rows that do see such a value get it added
 // to their output at the end.
 //
-// Every wait on an mbarrier gives up after 1 s, sets bit 0 of the plan's
-// status word, frees the TMEM and returns.
+// Every wait on an mbarrier gives up after 1 s; the CTA then sets bit 0 of the
+// plan's status word, frees the TMEM, fills its rows with NaN and returns.  A
+// plan whose status word is set gives NaN until it is cleared: what such a call
+// left in its outputs and workspace must not pass for a result.
 //
 // Measured, and what bounds it (copy 6.5 TB/s, matrix product 1,679 TFLOP/s):
 // - 6,496 frame-causal queries, 24 heads of 128, history merged (319 GFLOP):
@@ -250,6 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + kBarCount);
   volatile uint32_t* abort_flag = tslot + 1;
   volatile uint32_t* dirty_flag = tslot + 2;  // some V value was zeroed in this CTA
+  volatile uint32_t* failed_flag = tslot + 3;  // the plan's status word at the start
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.launch_dependents;");  // the merge may take SMs that have nothing left to do
   const int G = a.G;
@@ -493,6 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kScrubWarp) {
     // ----------------------------------------------------------- V scrub
+    if (lane == 0) *failed_flag = *static_cast<const volatile uint32_t*>(a.status);
     uint32_t vt = 0;
 #pragma unroll 1
     for (int i = first; i < last && ok; ++i) {
@@ -819,6 +823,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_after();
   if (*abort_flag && tid == 0) atomicOr(a.status, 1u);
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  if (*abort_flag | *failed_flag) {
+    // NaN for all of this CTA's rows (a part's maximum and sum carry it through the merge)
+    const float nan = __int_as_float(0x7FFFFFFF);
+#pragma unroll 1
+    for (int i = first; i < last; ++i) {
+      const PackedItem it = read_item(a.items + i);
+#pragma unroll 1
+      for (int r = warp; r < it.rows; r += kThreads / 32) {
+        const int tok = (it.row0 + r) / G, h = it.kvh * G + (it.row0 + r) - tok * G;
+        const int64_t q = int64_t(it.q_start) + tok;
+        if (it.part_row >= 0) {
+          if (lane == 0) reinterpret_cast<float2*>(a.part_ml)[int64_t(it.part_row) + r] = make_float2(nan, nan);
+          continue;
+        }
+        if (lane == 0) a.lse[int64_t(h) * a.lse_head + q] = nan;
+#pragma unroll 1
+        for (int c = lane; c < a.D; c += 32) {
+          const int64_t at = (q * a.H + h) * a.D + c;
+          if (a.out_f32) static_cast<float*>(a.out)[at] = nan;
+          else static_cast<uint16_t*>(a.out)[at] = uint16_t(0x7FFFu);
+        }
+      }
+    }
+  }
 }
 
 // The merge of a split unit's partial rows (and the history part), one warp

@@ -233,6 +233,7 @@ SIGNATURES = {
     "nkv_attend_plan_destroy": (C.c_int, [P]),
     "nkv_attend_plan_get_info": (C.c_int, [P, C.POINTER(nkv_attend_plan_info)]),
     "nkv_attend_plan_status": (C.c_int, [P, C.POINTER(C.c_uint32)]),
+    "nkv_attend_plan_set_status": (C.c_int, [P, C.c_uint32]),
     "nkv_attend_schedule": (C.c_int, [C.POINTER(U64), C.POINTER(U64), U64, I32, I32, I32, U64, I32, P, U64,
                                       C.POINTER(U64)]),
     "nkv_attend_packed": (C.c_int, [P, P, P]),

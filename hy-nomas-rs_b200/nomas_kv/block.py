@@ -506,10 +506,12 @@ class AttendPlan:
 
     def check(self) -> None:
         """Wait for the device and raise CudaError if a call of this plan gave
-        up on one of its bounded waits."""
+        up on one of its bounded waits since the last check.  From such a call
+        on the plan's results are NaN, until check has reported it."""
         w = C.c_uint32()
         _check(lib().nkv_attend_plan_status(self._h, C.byref(w)))
         if w.value:
+            _check(lib().nkv_attend_plan_set_status(self._h, 0))
             raise CudaError("packed attention: a bounded wait ran out")
 
 

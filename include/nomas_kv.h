@@ -555,10 +555,14 @@ int nkv_attend_plan_create(const uint64_t* q_lens, const uint64_t* k_lens, uint6
                            nkv_attend_plan** out);
 int nkv_attend_plan_destroy(nkv_attend_plan* plan);
 int nkv_attend_plan_get_info(const nkv_attend_plan* plan, nkv_attend_plan_info* out);
-/* Waits for the plan's device and reads the status word: bit 0 is set for
- * good once a bounded wait inside a call ran out (its outputs are then
- * undefined). */
+/* Waits for the plan's device and reads the status word: bit 0 is set once a
+ * bounded wait inside a call ran out.  The rows that call did not finish are
+ * NaN, and so is every row of the plan's later calls until the word is set back
+ * to 0. */
 int nkv_attend_plan_status(const nkv_attend_plan* plan, uint32_t* status);
+/* Waits for the plan's device and writes the status word (0: the failure has
+ * been dealt with). */
+int nkv_attend_plan_set_status(nkv_attend_plan* plan, uint32_t status);
 /* The plan's work list for `sms` SMs without a device: per item {sequence
  * start in q, in k, first packed row, rows, key/value head, first tile, last
  * tile + 1, first partial row or -1}; min(*n, cap) items written. */
