@@ -70,7 +70,12 @@ def _binding() -> None:
         return
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError as e:
+        # without torch nothing can call the block operators of nomas_kv
+        print(f"{e}: _block_binding.so not built", file=sys.stderr)
+        return
 
     base = os.path.dirname(torch.__file__)
     inc = [os.path.join(ROOT, "include"), os.path.join(base, "include"), sysconfig.get_paths()["include"],
@@ -79,7 +84,10 @@ def _binding() -> None:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in inc), src,
            "-o", BINDING, f"-L{os.path.join(base, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda",
            "-lc10"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as e:
+        raise RuntimeError(f"{e}: _block_binding.so needs a C++ compiler (CXX, default g++)") from e
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for block_binding.cpp:\n{r.stdout}\n{r.stderr}")
 
@@ -91,7 +99,6 @@ def build(clean: bool = False, verbose: bool = False) -> str:
     with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
         binding = ex.submit(_binding)
         objs = list(ex.map(_compile, SOURCES))
-        binding.result()
     if _newer(LIB, objs):
         cmd = [NVCC, "-shared", "-cudart", "static", "-gencode", "arch=compute_100a,code=sm_100a", "-o", LIB, *objs,
                "-lpthread", "-ldl", "-lrt"]
@@ -100,6 +107,9 @@ def build(clean: bool = False, verbose: bool = False) -> str:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     if verbose:
         print(LIB)
+    # last: the C library needs nvcc alone, and is there whether or not torch's
+    # headers, Python's and a C++ compiler are
+    binding.result()
     return LIB
 
 
