@@ -65,36 +65,58 @@ def _compile(src: str) -> str:
 
 
 def _binding() -> None:
-    src, header = os.path.join(CSRC, "block_binding.cpp"), os.path.join(ROOT, "include", "nomas_kv.h")
-    if not _newer(BINDING, [src, header]):
-        return
+    """_block_binding.so holds torch's and Python's internals as they were when it
+    was compiled: another version of either, or other flags, compile it anew."""
+    import importlib.metadata
+    import importlib.util
+    import json
     import sysconfig
 
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        # without torch nothing can call the block operators of nomas_kv
+        print("no torch: _block_binding.so not built", file=sys.stderr)
+        return
+    base = os.path.dirname(spec.origin)
+    src, header = os.path.join(CSRC, "block_binding.cpp"), os.path.join(ROOT, "include", "nomas_kv.h")
+    inc = [os.path.join(ROOT, "include"), os.path.join(base, "include"), sysconfig.get_paths()["include"],
+           os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-fPIC", "-O2", "-std=c++17", "-Wall", *(f"-isystem{i}" for i in inc),
+           src, "-o", BINDING, f"-L{os.path.join(base, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda",
+           "-lc10"]
+    stamp = os.path.join(BUILD, "block_binding.json")
+    made_for = json.dumps([importlib.metadata.version("torch"), sys.version, cmd]).replace(ROOT, "")
+    try:
+        with open(stamp) as f:
+            current = f.read() == made_for
+    except OSError:
+        current = False
+    if current and not _newer(BINDING, [src, header]):
+        return
+    if not current and os.path.exists(BINDING):
+        os.remove(BINDING)  # of another torch: not to be loaded, even if the compiler fails now
     try:
         import torch
     except ImportError as e:
-        # without torch nothing can call the block operators of nomas_kv
-        print(f"{e}: _block_binding.so not built", file=sys.stderr)
-        return
+        raise RuntimeError(f"_block_binding.so is compiled against torch: {e}") from e
 
-    base = os.path.dirname(torch.__file__)
-    inc = [os.path.join(ROOT, "include"), os.path.join(base, "include"), sysconfig.get_paths()["include"],
-           os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
-    cmd = [os.environ.get("CXX", "g++"), "-shared", "-fPIC", "-O2", "-std=c++17", "-Wall",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in inc), src,
-           "-o", BINDING, f"-L{os.path.join(base, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda",
-           "-lc10"]
+    cmd.insert(1, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}")
     try:
         r = subprocess.run(cmd, capture_output=True, text=True)
     except OSError as e:
         raise RuntimeError(f"{e}: _block_binding.so needs a C++ compiler (CXX, default g++)") from e
     if r.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed for block_binding.cpp:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(made_for)
 
 
 def build(clean: bool = False, verbose: bool = False) -> str:
-    if clean and os.path.isdir(BUILD):
-        shutil.rmtree(BUILD)
+    if clean:
+        shutil.rmtree(BUILD, ignore_errors=True)
+        for made in (LIB, BINDING):
+            if os.path.exists(made):
+                os.remove(made)
     os.makedirs(BUILD, exist_ok=True)
     with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as ex:
         binding = ex.submit(_binding)

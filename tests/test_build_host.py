@@ -62,3 +62,50 @@ def test_without_torch_there_is_the_c_library(build, monkeypatch, capsys):
     build.build()
     assert os.path.exists(build.LIB) and not os.path.exists(build.BINDING)
     assert "not built" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("change", ["torch", "python", "compiler"])
+def test_the_binding_is_compiled_anew_for_another_torch_or_python(build, monkeypatch, change):
+    import importlib.metadata
+    build.build()
+    build.ran.clear()
+    if change == "torch":
+        real = importlib.metadata.version
+        monkeypatch.setattr(importlib.metadata, "version", lambda n: "0.0.0+other" if n == "torch" else real(n))
+    elif change == "python":
+        monkeypatch.setattr(sys, "version", "3.99 (another)")
+    else:
+        monkeypatch.setenv("CXX", "another-c++")
+    build.build()
+    assert build.ran == ["_block_binding.so"]
+    build.ran.clear()
+    build.build()
+    assert build.ran == []
+
+
+def test_a_stale_binding_does_not_outlive_a_failed_compile(build, monkeypatch):
+    build.build()
+    monkeypatch.setattr(sys, "version", "3.99 (another)")
+    build.refuse = lambda cmd: "no" if _is_binding(cmd) else None
+    with pytest.raises(RuntimeError):
+        build.build()
+    assert not os.path.exists(build.BINDING)
+
+
+def test_a_failed_compile_is_tried_again(build):
+    build.refuse = lambda cmd: "no" if _is_binding(cmd) else None
+    for _ in range(2):
+        with pytest.raises(RuntimeError):
+            build.build()
+    build.refuse = lambda cmd: None
+    build.ran.clear()
+    build.build()
+    assert build.ran == ["_block_binding.so"]
+
+
+def test_clean_builds_everything_again(build):
+    build.build()
+    first = sorted(build.ran)
+    build.ran.clear()
+    build.build(clean=True)
+    assert sorted(build.ran) == first
