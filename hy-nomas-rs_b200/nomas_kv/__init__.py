@@ -14,7 +14,9 @@ kernels, and there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import math
+import os
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
@@ -28,12 +30,15 @@ __all__ = [
     "HistorySampling", "CacheStorage", "QvgConfig", "CacheConfig", "SegmentKv", "SegmentLayout", "CacheMetrics",
     "KvBank", "LayerCache", "build_cache", "history_frame_indices", "uniform_frame_indices",
     "recent_mix_uniform_frame_indices", "temporal_context_frame_indices", "plan_recent_trim", "partition_layers",
-    "lib", "RotaryAxes", "rope_tables", "rotary", "residual_norm", "AttendPlan", "attend_packed",
+    "lib",
 ]
 
 # the operators of block.py, imported at their first use: they need torch,
 # which the cache API itself only imports when a call does
 _BLOCK = ("RotaryAxes", "rope_tables", "rotary", "residual_norm", "AttendPlan", "attend_packed")
+# ("import *" fetches every name: those only where they can be had)
+if importlib.util.find_spec("torch") and os.path.exists(os.path.join(os.path.dirname(__file__), "_block_binding.so")):
+    __all__ += _BLOCK
 
 
 def __getattr__(name):
@@ -43,6 +48,10 @@ def __getattr__(name):
             globals()[n] = getattr(block, n)
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted({*globals(), *_BLOCK})
 
 
 # ------------------------------------------------------------------ errors

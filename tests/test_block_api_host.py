@@ -1,5 +1,33 @@
 """CPU checks of the block operators' entry points."""
+import os
+import subprocess
+import sys
+
+PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hy-nomas-rs_b200")
 
 
 def test_plan_set_status_refuses_a_null_plan(nkv):
     assert nkv.lib().nkv_attend_plan_set_status(None, 0) == 6
+
+
+def test_import_star_needs_no_torch():
+    """The cache API alone: torch and the compiled binding are needed by the block operators, at their first use."""
+    code = ("import sys; sys.modules['torch'] = None; sys.path.insert(0, sys.argv[1])\n"
+            "from nomas_kv import *\n"
+            "import nomas_kv\n"
+            "assert KvBank is nomas_kv.KvBank and 'AttendPlan' in dir(nomas_kv)\n"
+            "try:\n    nomas_kv.AttendPlan\nexcept ImportError: pass\nelse: raise SystemExit('no error')\n")
+    subprocess.run([sys.executable, "-c", code, PKG], check=True)
+
+
+def test_import_star_brings_the_block_operators_with_torch(nkv):
+    code = ("import sys; sys.path.insert(0, sys.argv[1])\n"
+            "from nomas_kv import *\n"
+            "import nomas_kv\n"
+            "assert AttendPlan is nomas_kv.AttendPlan and attend_packed and KvBank\n")
+    subprocess.run([sys.executable, "-c", code, PKG], check=True)
+
+
+def test_block_names_are_reached_through_the_package(nkv):
+    for name in ("RotaryAxes", "rope_tables", "rotary", "residual_norm", "AttendPlan", "attend_packed"):
+        assert getattr(nkv, name) is getattr(nkv.block, name) and name in dir(nkv)
