@@ -121,6 +121,12 @@ PyObject* handed(PyObject* given, at::Tensor& made) {  // a new reference
   return given;
 }
 
+// A write to a caller's output, counted as torch's in-place operations do: a
+// backward pass that saved it raises.
+void written(const at::Tensor* given) {
+  if (given && !given->is_inference()) given->unsafeGetTensorImpl()->bump_version();
+}
+
 void* address(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
 // A Python number; false (and no error set) if it is none.
@@ -228,6 +234,7 @@ PyObject* rope_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                      st);
         }))
       return nullptr;
+    written(given[0]), written(given[1]);
     return pair_of(handed(a[2], made[0]), handed(a[3], made[1]));
   });
 }
@@ -282,6 +289,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (k) r.k = side(*k, kw, ko, out[1]);
     void* st = in.stream();
     if (!run([&] { return entries.rotary(&r, st); })) return nullptr;
+    written(qo), written(ko);
     PyObject* first = handed(a[8], out[0]);
     return k ? pair_of(first, handed(a[9], out[1])) : first;
   });
@@ -363,6 +371,7 @@ PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     r.mod_rows = int32_t(groups);
     void* st = in.stream();
     if (!run([&] { return entries.residual_norm(&r, st); })) return nullptr;
+    written(ho), written(yo);
     PyObject* first = a[0];
     if (branch) first = handed(a[11], h);
     else Py_INCREF(first);
@@ -443,6 +452,7 @@ PyObject* attend_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* st = in.stream();
     if (!run([&] { return entries.attend_packed(reinterpret_cast<const nkv_attend_plan*>(plan.plan), &r, st); }))
       return nullptr;
+    written(out), written(lse);
     return pair_of(handed(a[7], made), handed(a[8], made_lse));
   });
 }

@@ -197,6 +197,14 @@ def _check_out(out, like, ins, name: str, alias=(), others=()):
         raise ArgumentError(f"{name} overlaps another output")
 
 
+def _written(*given) -> None:
+    """Counts the write to the caller's outputs, as torch's in-place operations
+    do: a backward pass that saved one of them raises."""
+    for t in given:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 # ---------------------------------------------------------------- rotary
 @dataclass(frozen=True)
 class RotaryAxes:
@@ -250,6 +258,7 @@ def rope_tables(positions, axes: RotaryAxes, cos=None, sin=None, stream=None):
     index = _device_of(positions, cos, sin)
     code = _positions(positions, axes, None)
     shape = (positions.shape[0], axes.pairs)
+    given = (cos, sin)
     away = _enter(index, stream, (positions, cos, sin))
     try:
         for name, t, other in (("cos", cos, sin), ("sin", sin, cos)):
@@ -266,6 +275,7 @@ def rope_tables(positions, axes: RotaryAxes, cos=None, sin=None, stream=None):
     finally:
         if away is not None:
             away.leave()
+    _written(*given)
     return cos, sin
 
 
@@ -309,6 +319,7 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
             raise GeometryError(f"{name} must be a contiguous ({D},) {q.dtype} tensor")
     ins = (q, k, positions, q_weight, k_weight)
     apart = k is q  # read as both: neither may be rotated in place
+    given = (q_out, k_out)
     away = _enter(index, stream, (*ins, q_out, k_out))
     try:
         if q_out is not None:
@@ -336,6 +347,7 @@ def rotary(positions, axes: RotaryAxes, q, k=None, norm: bool = False, q_weight=
     finally:
         if away is not None:
             away.leave()
+    _written(*given)
     return q_out if k is None else (q_out, k_out)
 
 
@@ -438,6 +450,7 @@ def residual_norm(x, branch=None, *, gate=None, post=None, post_weight=None, nor
     finally:
         if away is not None:
             away.leave()
+    _written(h_out, y_out)
     return h, y
 
 
@@ -569,6 +582,7 @@ def attend_packed(plan: AttendPlan, q, k, v, scale: Optional[float] = None, hist
             if t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous():
                 raise GeometryError(f"the history's {name} must be a contiguous f32 tensor of shape {shape}")
         ho_p, hl_p = ho.data_ptr(), hl.data_ptr()
+    given = (out, lse)
     away = _enter(index, stream, (q, k, v, ho, hl, out, lse))
     try:
         padded = rows != plan.q_tokens
@@ -597,4 +611,5 @@ def attend_packed(plan: AttendPlan, q, k, v, scale: Optional[float] = None, hist
     finally:
         if away is not None:
             away.leave()
+    _written(*given)
     return out, lse
