@@ -381,20 +381,38 @@ class LayerCache:
         (modules/attention.rs:143-189): softmax over this layer's history,
         which every query sees, and the current segment's k / v as `plan` (an
         AttendPlan) masks them.  q (plan.q_tokens, H, 128), k / v
-        (plan.k_tokens, H / group, 128) bf16 on the bank's device and stream;
-        returns (out, lse) of attend_packed.  The history part runs through
-        attend_history and its conditions apply (INT8 storage); an empty
-        history leaves the current segment alone."""
+        (plan.k_tokens, H / group, 128) bf16 on the bank's device; returns
+        (out, lse) of attend_packed.  It runs on the bank's stream; called on
+        another one, it waits for that one's work so far, and that one for
+        it.  The history part runs through attend_history and its conditions
+        apply (INT8 storage); an empty history leaves the current segment
+        alone."""
         from . import block
         b = self._bank
         if plan.heads != b.heads or plan.head_dim != b.head_dim:
             raise GeometryError(f"the plan must have {b.heads} heads of {b.head_dim}")
         torch = _torch()
-        with torch.cuda.stream(b.stream):
-            history = None
-            if self.valid_len():
-                history = self.attend_history(q, scale)
-            return block.attend_packed(plan, q, k, v, scale=scale, history=history, out=out, lse=lse)
+        stream = b.stream
+        caller = torch.cuda.current_stream(stream.device)
+        other = caller != stream
+        if other:
+            stream.wait_stream(caller)
+        try:
+            with torch.cuda.stream(stream):
+                history = None
+                if self.valid_len():
+                    history = self.attend_history(q, scale)
+                result = block.attend_packed(plan, q, k, v, scale=scale, history=history, out=out, lse=lse)
+        finally:
+            if other:
+                caller.wait_stream(stream)
+                for t in (q, k, v, out, lse):  # the caller's memory, in use on the bank's stream
+                    if t is not None and t.is_cuda:
+                        t.record_stream(stream)
+        if other:
+            for t in result:  # and the other way round
+                t.record_stream(caller)
+        return result
 
     # QvgCodec::with_codebooks (qvg.rs:101-104) / codebooks readback
     def set_qvg_codebooks(self, cb) -> None:
