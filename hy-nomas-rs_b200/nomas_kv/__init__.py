@@ -363,6 +363,8 @@ class LayerCache:
         b = self._bank
         if q.dim() != 3 or q.shape[1:] != (b.heads, b.head_dim) or q.dtype != torch.bfloat16 or not q.is_contiguous():
             raise GeometryError(f"q must be a contiguous (q_len, {b.heads}, {b.head_dim}) bf16 tensor")
+        if q.device != b.stream.device:
+            raise ArgumentError(f"q must be on {b.stream.device}, where the bank is, not on {q.device}")
         n = q.shape[0]
         if out is None:
             out = torch.empty((n, b.heads, b.head_dim), dtype=torch.float32, device=q.device)

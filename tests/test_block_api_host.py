@@ -1,7 +1,11 @@
 """CPU checks of the block operators' entry points."""
+import contextlib
 import os
 import subprocess
 import sys
+from types import SimpleNamespace
+
+import pytest
 
 PKG = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hy-nomas-rs_b200")
 
@@ -31,3 +35,31 @@ def test_import_star_brings_the_block_operators_with_torch(nkv):
 def test_block_names_are_reached_through_the_package(nkv):
     for name in ("RotaryAxes", "rope_tables", "rotary", "residual_norm", "AttendPlan", "attend_packed"):
         assert getattr(nkv, name) is getattr(nkv.block, name) and name in dir(nkv)
+
+
+@pytest.mark.parametrize("call", ["attend_history", "attend"])
+def test_history_attention_refuses_tensors_elsewhere(nkv, monkeypatch, call):
+    """An address of another device (or the host's) must not reach a kernel."""
+    import torch
+    reached = []
+
+    class Lib:
+        def __getattr__(self, name):
+            def f(*a):
+                reached.append(name)
+                return 0
+            return f
+
+    monkeypatch.setattr(nkv, "lib", Lib)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: stream)
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    monkeypatch.setattr(nkv.LayerCache, "valid_len", lambda self: 4)
+    stream = SimpleNamespace(device=torch.device("cuda", 0))
+    layer = nkv.LayerCache(SimpleNamespace(heads=2, head_dim=128, stream=stream, _h=None), 0)
+    q = torch.zeros((4, 2, 128), dtype=torch.bfloat16)
+    with pytest.raises(nkv.ArgumentError, match="cuda:0"):
+        if call == "attend":
+            layer.attend(SimpleNamespace(heads=2, head_dim=128), q, q, q)
+        else:
+            layer.attend_history(q)
+    assert "nkv_bank_attend_history" not in reached
