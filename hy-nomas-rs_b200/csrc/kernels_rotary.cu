@@ -284,7 +284,8 @@ __global__ void __launch_bounds__(kVecThreads, 5) k_rotary_vec(const RotaryParam
   //   a' = a (w_a c) - b (w_b s),  b' = b (w_b c) + a (w_a s),
   // on two pairs at a time.  A pair that passes through is only multiplied by
   // its gains: its partner is masked to 0 (a sine of 0 alone would turn an
-  // infinite partner into a NaN).
+  // infinite partner into a NaN) and its sine to -0 (0 * -0 + x is x, for x = -0
+  // too).
   float2 cs[8];
   uint32_t mask[8];
   bool all = true;
@@ -329,8 +330,8 @@ __global__ void __launch_bounds__(kVecThreads, 5) k_rotary_vec(const RotaryParam
         ca[j] = make_float2(a0 * u.x, a1 * v.x);
         cb[j] = make_float2(b0 * u.x, b1 * v.x);
         const bool r0 = kAll || mask[2 * j], r1 = kAll || mask[2 * j + 1];
-        sb[j] = make_float2(r0 ? -b0 * u.y : 0.0f, r1 ? -b1 * v.y : 0.0f);
-        sa[j] = make_float2(r0 ? a0 * u.y : 0.0f, r1 ? a1 * v.y : 0.0f);
+        sb[j] = make_float2(r0 ? -b0 * u.y : -0.0f, r1 ? -b1 * v.y : -0.0f);
+        sa[j] = make_float2(r0 ? a0 * u.y : -0.0f, r1 ? a1 * v.y : -0.0f);
       }
       uintptr_t dst = first_row(S.out, S.out_token, S.out_head);
       const int64_t dst_step = S.out_head * kSize << a.log_hp;

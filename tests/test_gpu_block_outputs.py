@@ -1,4 +1,4 @@
-"""Outputs that a caller gives to the block operators."""
+"""Outputs that a caller gives to the block operators, and values that they pass through."""
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +58,23 @@ def test_inference_tensors_are_taken(nkv, path):
         assert all(t.is_inference() for t in written)
         call()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("layout", ["aligned", "odd"])
+def test_values_past_the_rotated_ones_pass_through(nkv, dtype, interleaved, layout):
+    """Bit for bit: zeros of either sign, infinities, subnormals."""
+    import torch
+    dt, T, H, D, R = getattr(torch, dtype), 9, 3, 64, 32
+    x = torch.randn((T, H, D + 1), device="cuda").to(dt)
+    x = x[..., 1:] if layout == "odd" else x[..., 1:].contiguous()
+    x[..., R::4] = 0.0
+    x[..., R + 1::4] = -0.0
+    x[..., R + 2::8] = float("inf")
+    x[..., R + 6::8] = torch.finfo(dt).smallest_normal / 4
+    pos = torch.randint(1, 50, (T, 1), dtype=torch.int32, device="cuda")
+    out = nkv.rotary(pos, nkv.RotaryAxes((R,), interleaved=interleaved), x)
+    whole = {2: torch.int16, 4: torch.int32}[x.element_size()]
+    assert torch.equal(out[..., R:].contiguous().view(whole), x[..., R:].contiguous().view(whole))
+    assert bool(out[..., :R].isfinite().all())
