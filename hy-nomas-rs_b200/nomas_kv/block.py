@@ -459,6 +459,8 @@ def _lens(v: Sequence[int], name: str):
     v = [int(n) for n in v]
     if any(n < 0 for n in v):
         raise GeometryError(f"{name} must not be negative")
+    if any(n >= 2 ** 31 for n in v):  # (before ctypes takes them modulo 2^64)
+        raise GeometryError("sequence too long")
     return v, (C.c_uint64 * max(len(v), 1))(*v)
 
 
@@ -481,10 +483,12 @@ class AttendPlan:
         k, ka = (q, qa) if k_lens is None else _lens(k_lens, "k_lens")
         if len(q) != len(k):
             raise GeometryError("q_lens and k_lens must have one entry per sequence")
-        if int(block) < 1:
+        if not 1 <= int(block) < 2 ** 31:
             raise ArgumentError("block must be 1 to 2^31 - 1")
         self.heads, self.kv_heads = int(heads), int(heads if kv_heads is None else kv_heads)
         self.head_dim, self.causal, self.block = int(head_dim), bool(causal), int(block)
+        if any(abs(n) >= 2 ** 31 for n in (self.heads, self.kv_heads, self.head_dim)):
+            raise GeometryError("heads, kv_heads and head_dim must fit in 32 bits")
         if device is None:
             device = torch.device("cuda", torch.cuda.current_device() if torch.cuda.is_available() else 0)
         device = torch.device(device)

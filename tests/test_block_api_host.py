@@ -63,3 +63,26 @@ def test_history_attention_refuses_tensors_elsewhere(nkv, monkeypatch, call):
         else:
             layer.attend_history(q)
     assert "nkv_bank_attend_history" not in reached
+
+
+@pytest.mark.parametrize("change", [dict(q_lens=[2 ** 64 + 1]), dict(k_lens=[2 ** 64 + 5]), dict(block=2 ** 64 + 1),
+                                    dict(heads=2 ** 32 + 4), dict(kv_heads=2 ** 32 + 4), dict(head_dim=2 ** 32 + 64),
+                                    dict(heads=-2 ** 32 + 4)])
+def test_plan_refuses_numbers_that_do_not_fit(nkv, monkeypatch, change):
+    """2^64 + 1 must not be taken for 1: such a plan would be another one than was asked for."""
+    made = []
+
+    class Lib:
+        def nkv_attend_plan_create(self, *a):
+            made.append(a)
+            raise nkv.CudaError("reached")
+
+    from nomas_kv import block
+    monkeypatch.setattr(block, "lib", Lib)
+    with pytest.raises(nkv.CudaError, match="reached"):  # what fits gets there
+        nkv.AttendPlan([1], 4, kv_heads=4, head_dim=64, k_lens=[5], device="cuda:0")
+    made.clear()
+    args = dict(dict(q_lens=[1], heads=4, kv_heads=4, head_dim=64, k_lens=[5], device="cuda:0"), **change)
+    with pytest.raises((nkv.GeometryError, nkv.ArgumentError)):
+        nkv.AttendPlan(args.pop("q_lens"), args.pop("heads"), **args)
+    assert not made
