@@ -44,8 +44,8 @@
 //
 // Measured, and what bounds it (copy 6.5 TB/s, matrix product 1,679 TFLOP/s):
 // - 6,496 frame-causal queries, 24 heads of 128, history merged (319 GFLOP):
-//   300 to 350 us by the GPU's power limit (clock down to 1,650 MHz), 0.9 to
-//   1.05 PFLOP/s; tensor pipe 59 %, issue 52 %: the softmax warps' chain of
+//   295 to 355 us by the GPU's power limit (clock down to 1,650 MHz), 0.9 to
+//   1.08 PFLOP/s; tensor pipe 59 %, issue 52 %: the softmax warps' chain of
 //   latencies per step (about 1,450 cycles for both halves, 1,280 of them tensor
 //   time at head_dim 128: S at N = 64 takes 48 cycles per MMA, bound by shared
 //   memory, where N = 128 would need 512 more TMEM columns).
@@ -156,6 +156,35 @@ __device__ __forceinline__ PackedItem read_item(const PackedItem* p) {
   return it;
 }
 
+// NaN for all rows of the items first .. last - 1 (a part's maximum and sum
+// carry it through the merge).  Not inlined: the steps' registers would be dealt
+// out anew (six prompts of f16 217 us instead of 214, 8 bytes of spills at
+// head_dim 64).
+__device__ __noinline__ void fill_nan(const PackedArgs* a, int first, int last) {
+  const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31, G = a->G;
+  const float nan = __int_as_float(0x7FFFFFFF);
+#pragma unroll 1
+  for (int i = first; i < last; ++i) {
+    const PackedItem it = read_item(a->items + i);
+#pragma unroll 1
+    for (int r = warp; r < it.rows; r += kThreads / 32) {
+      const int tok = (it.row0 + r) / G, h = it.kvh * G + (it.row0 + r) - tok * G;
+      const int64_t q = int64_t(it.q_start) + tok;
+      if (it.part_row >= 0) {
+        if (lane == 0) reinterpret_cast<float2*>(a->part_ml)[int64_t(it.part_row) + r] = make_float2(nan, nan);
+        continue;
+      }
+      if (lane == 0) a->lse[int64_t(h) * a->lse_head + q] = nan;
+#pragma unroll 1
+      for (int c = lane; c < a->D; c += 32) {
+        const int64_t at = (q * a->H + h) * a->D + c;
+        if (a->out_f32) static_cast<float*>(a->out)[at] = nan;
+        else static_cast<uint16_t*>(a->out)[at] = uint16_t(0x7FFFu);
+      }
+    }
+  }
+}
+
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return DT == BF16 ? dev::bf16x2_bits_nonnan(a, b) : dev::f16x2_bits_nonnan(a, b);
@@ -236,7 +265,7 @@ template <int DT, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     k_attend_packed(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                     const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap hmap,
-                    const PackedArgs a) {
+                    const __grid_constant__ PackedArgs a) {
   using Sh = Shape<DP>;
   constexpr int NST = Sh::kStages;
   extern __shared__ unsigned char packed_raw[];
@@ -823,30 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_after();
   if (*abort_flag && tid == 0) atomicOr(a.status, 1u);
   if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-  if (*abort_flag | *failed_flag) {
-    // NaN for all of this CTA's rows (a part's maximum and sum carry it through the merge)
-    const float nan = __int_as_float(0x7FFFFFFF);
-#pragma unroll 1
-    for (int i = first; i < last; ++i) {
-      const PackedItem it = read_item(a.items + i);
-#pragma unroll 1
-      for (int r = warp; r < it.rows; r += kThreads / 32) {
-        const int tok = (it.row0 + r) / G, h = it.kvh * G + (it.row0 + r) - tok * G;
-        const int64_t q = int64_t(it.q_start) + tok;
-        if (it.part_row >= 0) {
-          if (lane == 0) reinterpret_cast<float2*>(a.part_ml)[int64_t(it.part_row) + r] = make_float2(nan, nan);
-          continue;
-        }
-        if (lane == 0) a.lse[int64_t(h) * a.lse_head + q] = nan;
-#pragma unroll 1
-        for (int c = lane; c < a.D; c += 32) {
-          const int64_t at = (q * a.H + h) * a.D + c;
-          if (a.out_f32) static_cast<float*>(a.out)[at] = nan;
-          else static_cast<uint16_t*>(a.out)[at] = uint16_t(0x7FFFu);
-        }
-      }
-    }
-  }
+  if (*abort_flag | *failed_flag) fill_nan(&a, first, last);
 }
 
 // The merge of a split unit's partial rows (and the history part), one warp
