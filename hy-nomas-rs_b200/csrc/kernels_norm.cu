@@ -343,9 +343,10 @@ __device__ __forceinline__ void put_row(void* p, int64_t base, int n, int thread
     if (k < n) put<DT>(p, at + k * threads, v[k]);
 }
 
-// Any dim and any alignment (what k_residual_norm_vec cannot take: where both
-// can, 6,496 rows of 5,120 columns take 152 us here, 52 there; of 128 columns 9
-// and 8): blockDim.x threads per row, each holding the E
+// Any dim and any alignment (what k_residual_norm_vec cannot take, rows above
+// 8,192 columns among it: where both can, 6,496 rows of 5,120 columns take 152
+// us here, 52 there; of 128 columns 9 and 8).  One value per load and up to five
+// waits for memory or a barrier in turn bound it: blockDim.x threads per row, each holding the E
 // values tid, tid + blockDim.x, ...; one row per CTA, or one per warp when 32
 // threads suffice.  Up to 2,048 columns at 40 registers, for more rows at once
 // (6,000 rows of 2,047: 53 us; at 48 58, at 32 54).
