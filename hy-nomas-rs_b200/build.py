@@ -73,7 +73,7 @@ def _binding() -> None:
     import sysconfig
 
     spec = importlib.util.find_spec("torch")
-    if spec is None:
+    if spec is None or not spec.origin:  # (a folder of that name has no origin)
         # without torch nothing can call the block operators of nomas_kv
         print("no torch: _block_binding.so not built", file=sys.stderr)
         return
@@ -85,7 +85,11 @@ def _binding() -> None:
            src, "-o", BINDING, f"-L{os.path.join(base, 'lib')}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda",
            "-lc10"]
     stamp = os.path.join(BUILD, "block_binding.json")
-    made_for = json.dumps([importlib.metadata.version("torch"), sys.version, cmd]).replace(ROOT, "")
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:  # a source tree: its version file says when it was built
+        version = os.path.getmtime(os.path.join(base, "version.py"))
+    made_for = json.dumps([version, sys.version, cmd]).replace(ROOT, "")
     try:
         with open(stamp) as f:
             current = f.read() == made_for

@@ -37,7 +37,7 @@ __all__ = [
 # which the cache API itself only imports when a call does
 _BLOCK = ("RotaryAxes", "rope_tables", "rotary", "residual_norm", "AttendPlan", "attend_packed")
 # ("import *" fetches every name: those only where they can be had)
-if importlib.util.find_spec("torch") and os.path.exists(os.path.join(os.path.dirname(__file__), "_block_binding.so")):
+if getattr(importlib.util.find_spec("torch"), "origin", None) and os.path.exists(os.path.join(os.path.dirname(__file__), "_block_binding.so")):
     __all__ += _BLOCK
 
 

@@ -83,6 +83,31 @@ def test_the_binding_is_compiled_anew_for_another_torch_or_python(build, monkeyp
     assert build.ran == []
 
 
+def test_torch_without_package_metadata(build, monkeypatch):
+    """A source build on the path: its version file stands for the version."""
+    import importlib.metadata
+
+    def version(name):
+        raise importlib.metadata.PackageNotFoundError(name)
+
+    monkeypatch.setattr(importlib.metadata, "version", version)
+    build.build()
+    assert os.path.exists(build.BINDING)
+    build.ran.clear()
+    build.build()
+    assert build.ran == []
+
+
+def test_a_folder_named_torch_is_not_torch(build, monkeypatch, tmp_path):
+    import importlib.util
+    from importlib.machinery import ModuleSpec
+    real = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec",
+                        lambda n, *a: ModuleSpec(n, None, is_package=True) if n == "torch" else real(n, *a))
+    build.build()
+    assert os.path.exists(build.LIB) and not os.path.exists(build.BINDING)
+
+
 def test_a_stale_binding_does_not_outlive_a_failed_compile(build, monkeypatch):
     build.build()
     monkeypatch.setattr(sys, "version", "3.99 (another)")
